@@ -1,4 +1,6 @@
-"""B200-native (sm_100a) fused 2D-RoPE + varlen attention forward.
+"""B200-native (sm_100a) fused 2D-RoPE + varlen attention, and the operators of the
+transformer block around it (layer norm, linear layer with epilogue, 8-bit
+activation checkpoints).
 
 Drop-in for the reference module ``fused_attn`` of sdan/fused-rope-attn
 (``fused_rope_attention``, ``compute_rope_2d``) and its ``utils``
@@ -16,6 +18,18 @@ from .fused_attn import (  # noqa: F401
     next_pow2,
     qkv_rope_projection,
     rope_positions_2d,
+)
+from .block_ops import (  # noqa: F401
+    ACTIVATIONS,
+    PackedActivation,
+    layer_norm,
+    layer_norm_backward,
+    layer_norm_train,
+    linear_act,
+    linear_act_backward,
+    linear_act_train,
+    pack_activation,
+    unpack_activation,
 )
 
 __version__ = "0.1.0"

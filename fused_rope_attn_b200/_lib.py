@@ -25,6 +25,7 @@ STATUS_BAD_POSITIONS = 0x400
 
 # Every symbol include/frattn.h declares, with (restype, argtypes).
 _vp, _i, _sz, _u64, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_uint64, ctypes.c_float
+_ll = ctypes.c_longlong
 _SIGNATURES = {
     "frattn_version": (_i, []),
     "frattn_error_string": (ctypes.c_char_p, [_i]),
@@ -46,6 +47,18 @@ _SIGNATURES = {
     "frattn_workspace_bytes_fp8": (_i, [_i, _i, _i, _i, ctypes.POINTER(_sz)]),
     "frattn_fwd_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _sz, _vp, _vp]),
     "frattn_fwd_noalloc": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
+    "frattn_act_pack": (_i, [_vp, _ll, _i, _i, _i, _vp, _vp, _vp]),
+    "frattn_act_unpack": (_i, [_vp, _vp, _i, _i, _i, _vp, _ll, _vp]),
+    "frattn_layer_norm": (_i, [_vp, _ll, _vp, _vp, _i, _i, _i, _f, _i, _vp, _ll, _vp, _vp, _vp]),
+    "frattn_workspace_bytes_layer_norm_bwd": (_i, [_i, _i, ctypes.POINTER(_sz)]),
+    "frattn_layer_norm_bwd": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _ll, _vp, _vp,
+                                   _vp, _sz, _vp]),
+    "frattn_workspace_bytes_linear_act": (_i, [_i, _i, _i, ctypes.POINTER(_sz)]),
+    "frattn_linear_act": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _ll, _i, _i, _i, _i, _i, _vp, _ll, _vp, _ll, _vp, _vp,
+                               _vp, _sz, _vp, _vp]),
+    "frattn_workspace_bytes_linear_act_bwd": (_i, [_i, _i, _i, ctypes.POINTER(_sz)]),
+    "frattn_linear_act_bwd": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _i,
+                                   _vp, _ll, _vp, _vp, _vp, _sz, _vp, _vp]),
     "frattn_window_plan_sizes": (_i, [_vp, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_int64),
                                       ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(_sz)]),
     "frattn_window_plan": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _f, _vp, _sz, _vp]),
@@ -140,4 +153,25 @@ def workspace_bytes_fp8(total_tokens: int, num_segments: int, num_heads: int, he
     out = ctypes.c_size_t(0)
     check(load().frattn_workspace_bytes_fp8(int(total_tokens), int(num_segments), int(num_heads), int(head_dim),
                                             ctypes.byref(out)), "frattn_workspace_bytes_fp8")
+    return int(out.value)
+
+
+def workspace_bytes_layer_norm_bwd(total_tokens: int, width: int) -> int:
+    out = ctypes.c_size_t(0)
+    check(load().frattn_workspace_bytes_layer_norm_bwd(int(total_tokens), int(width), ctypes.byref(out)),
+          "frattn_workspace_bytes_layer_norm_bwd")
+    return int(out.value)
+
+
+def workspace_bytes_linear_act(total_tokens: int, k: int, n: int) -> int:
+    out = ctypes.c_size_t(0)
+    check(load().frattn_workspace_bytes_linear_act(int(total_tokens), int(k), int(n), ctypes.byref(out)),
+          "frattn_workspace_bytes_linear_act")
+    return int(out.value)
+
+
+def workspace_bytes_linear_act_bwd(total_tokens: int, k: int, n: int) -> int:
+    out = ctypes.c_size_t(0)
+    check(load().frattn_workspace_bytes_linear_act_bwd(int(total_tokens), int(k), int(n), ctypes.byref(out)),
+          "frattn_workspace_bytes_linear_act_bwd")
     return int(out.value)

@@ -1,0 +1,528 @@
+"""Transformer-block operators around the attention: layer norm, linear layer with
+bias, activation and residual in its epilogue, and 8-bit activation checkpoints.
+
+The reference (sdan/fused-rope-attn) has the attention alone, forward only
+(fused_attn.py:139-232). A block that is trained or served around it needs the
+operators here; each calls hand-written sm_100a kernels through the C ABI
+(include/frattn.h) on the current stream:
+
+* ``layer_norm`` / ``layer_norm_backward``; ``layer_norm_train`` records the pair
+  as an autograd node;
+* ``linear_act`` / ``linear_act_backward``; ``linear_act_train`` likewise;
+* ``pack_activation`` / ``unpack_activation``: a tensor kept for the backward pass
+  in 8 bits (blocks of 32 values with a power-of-two scale each). Both backward
+  passes take a ``PackedActivation`` in the place of the tensor it stands for, and
+  the autograd nodes keep their inputs that way with ``checkpoint=True``.
+
+Matrices are ``[T, C]`` with packed columns; rows may be strided (views of wider
+buffers are read in place).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .fused_attn import _DT, _aligned, _status_word
+
+__all__ = [
+    "ACTIVATIONS",
+    "PackedActivation",
+    "pack_activation",
+    "unpack_activation",
+    "layer_norm",
+    "layer_norm_backward",
+    "layer_norm_train",
+    "linear_act",
+    "linear_act_backward",
+    "linear_act_train",
+]
+
+PACK_BLOCK = 32
+
+# Values of the FRATTN_ACT_* enum of include/frattn.h.
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+class _on:
+    """``torch.cuda.device(dev)`` that costs nothing when dev is already current."""
+
+    __slots__ = ("ctx",)
+
+    def __init__(self, device):
+        self.ctx = None if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _check_rows(name, t, dtypes):
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on CUDA, got device={t.device}")
+    if t.ndim != 2:
+        raise ValueError(f"{name} must be 2D [T, C], got {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} dtype must be one of {', '.join(str(d)[6:] for d in dtypes)}, got {t.dtype}")
+    if t.shape[1] <= 0:
+        raise ValueError(f"{name} must have at least one column, got {tuple(t.shape)}")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t with packed columns (rows may be strided); copied when they are not."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t with rows that start on 16-byte boundaries (a TMA requirement): t itself, or a
+    copy in rows padded to a multiple of 8 elements. A weight whose width is not a
+    multiple of 8 is best kept that way by its owner (a ``[:, :K]`` view of a padded
+    buffer), so that no call copies it."""
+    n, k = t.shape
+    if ((t.stride(1) == 1 or k == 1) and t.data_ptr() % 16 == 0
+            and (n == 1 or t.stride(0) % 8 == 0 and t.stride(0) >= k)):
+        return t
+    return torch.empty(n, -(-k // 8) * 8, dtype=t.dtype, device=t.device)[:, :k].copy_(t)
+
+
+def _stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _check_out_rows(out, shape, like, name="out"):
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"{name} must be {tuple(shape)} {like.dtype} on {like.device}, "
+                         f"got {tuple(out.shape)} {out.dtype} on {out.device}")
+    if out.stride(1) != 1 and out.shape[1] > 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise ValueError(f"{name} must have packed columns and non-overlapping rows, got strides {out.stride()}")
+    return out
+
+
+# --------------------------------------------------------------------------- 8-bit checkpoints
+class PackedActivation(NamedTuple):
+    """An ``[T, width]`` tensor kept in 8 bits: ``codes`` int8 ``[T, 32 * nb]`` and
+    ``scales`` uint8 ``[T, nb]`` (biased exponents), ``nb = ceil(width / 32)``; ``dtype``
+    is the type of the tensor it stands for. A value is ``code * 2**(scale - 127)``;
+    a block that held an infinity or a NaN has scale 255 and stands for NaN."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    width: int
+    dtype: torch.dtype
+
+    @property
+    def shape(self):
+        return torch.Size((self.scales.shape[0], self.width))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def _check_packed(name, p, dtype=None, shape=None):
+    t, nb = p.scales.shape if p.scales.ndim == 2 else (-1, -1)
+    if nb != -(-p.width // PACK_BLOCK) or p.width <= 0 or tuple(p.codes.shape) != (t, nb * PACK_BLOCK):
+        raise ValueError(f"{name}: codes {tuple(p.codes.shape)} and scales {tuple(p.scales.shape)} do not hold "
+                         f"rows of {p.width} values in blocks of {PACK_BLOCK}")
+    if p.codes.dtype != torch.int8 or p.scales.dtype != torch.uint8 or p.codes.device != p.scales.device:
+        raise ValueError(f"{name}: codes must be int8 and scales uint8 on one device, got {p.codes.dtype} on "
+                         f"{p.codes.device} and {p.scales.dtype} on {p.scales.device}")
+    if p.codes.device.type != "cuda":
+        raise ValueError(f"{name} must be on CUDA, got device={p.codes.device}")
+    if not p.codes.is_contiguous() or not p.scales.is_contiguous() or p.codes.data_ptr() % 16:
+        raise ValueError(f"{name}: codes and scales must be contiguous, codes 16-byte aligned")
+    if shape is not None and tuple(p.shape) != tuple(shape):
+        raise ValueError(f"{name} must stand for {tuple(shape)}, got {tuple(p.shape)}")
+    if dtype is not None and p.dtype != dtype:
+        raise ValueError(f"{name} must stand for {dtype}, got {p.dtype}")
+
+
+def _empty_packed(rows, width, dtype, device) -> PackedActivation:
+    nb = -(-width // PACK_BLOCK)
+    return PackedActivation(torch.empty(rows, nb * PACK_BLOCK, dtype=torch.int8, device=device),
+                            torch.empty(rows, nb, dtype=torch.uint8, device=device), width, dtype)
+
+
+def pack_activation(x: torch.Tensor) -> PackedActivation:
+    """``x`` ``[T, C]`` (float32, float16 or bfloat16) in 8 bits: 1 + 1/32 bytes a value.
+
+    Per block of 32 columns with largest magnitude ``f * 2**q`` (1/2 <= f < 1) the step is
+    ``2**max(q - 7, -126)`` and each value is rounded to the nearest multiple of it
+    (ties to even; at most 127 steps)."""
+    _check_rows("x", x, tuple(_DT))
+    x = _rows(x)
+    p = _empty_packed(x.shape[0], x.shape[1], x.dtype, x.device)
+    with _on(x.device):
+        rc = _lib.load().frattn_act_pack(x.data_ptr(), _stride(x), x.shape[0], x.shape[1], _DT[x.dtype],
+                                         p.codes.data_ptr(), p.scales.data_ptr(), _stream(x.device))
+    _lib.check(rc, "frattn_act_pack")
+    return p
+
+
+def unpack_activation(p: PackedActivation, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values a checkpoint stands for, ``[T, width]`` of its dtype."""
+    _check_packed("packed activation", p)
+    if p.dtype not in _DT:
+        raise ValueError(f"dtype must be float16, bfloat16 or float32, got {p.dtype}")
+    if out is None:
+        out = torch.empty(p.shape, dtype=p.dtype, device=p.device)
+    else:
+        out = _check_out_rows(out, p.shape, torch.empty(0, dtype=p.dtype, device=p.device))
+    with _on(p.device):
+        rc = _lib.load().frattn_act_unpack(p.codes.data_ptr(), p.scales.data_ptr(), p.shape[0], p.width,
+                                           _DT[p.dtype], out.data_ptr(), _stride(out), _stream(p.device))
+    _lib.check(rc, "frattn_act_unpack")
+    return out
+
+
+# --------------------------------------------------------------------------- layer norm
+def _check_param(name, t, C, dtype, device):
+    if t.shape != (C,):
+        raise ValueError(f"{name} must be [{C}], got {tuple(t.shape)}")
+    if t.dtype not in (dtype, torch.float32):
+        raise ValueError(f"{name} dtype must be {dtype} or float32, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    return t.contiguous()
+
+
+def layer_norm(
+    x: torch.Tensor,
+    weight: torch.Tensor | None = None,
+    bias: torch.Tensor | None = None,
+    *,
+    eps: float = 1e-6,
+    out: torch.Tensor | None = None,
+    return_stats: bool = False,
+):
+    """Layer norm over the columns of ``x`` ``[T, C]`` (float32, float16 or bfloat16).
+
+    ``weight`` and ``bias`` ``[C]`` in x's type or float32 (both the same). With
+    ``return_stats`` also the fp32 ``mean`` and ``rstd`` ``[T]`` of the rows, which
+    ``layer_norm_backward`` takes.
+    """
+    _check_rows("x", x, tuple(_DT))
+    T, C = x.shape
+    if not eps >= 0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    weight = None if weight is None else _check_param("weight", weight, C, x.dtype, x.device)
+    bias = None if bias is None else _check_param("bias", bias, C, x.dtype, x.device)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"weight and bias must share a dtype, got {weight.dtype} and {bias.dtype}")
+    pd = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+    x = _rows(x)
+    out = _check_out_rows(out, (T, C), x)
+    mean = rstd = None
+    if return_stats:
+        mean, rstd = torch.empty(2, T, dtype=torch.float32, device=x.device).unbind(0)
+    with _on(x.device):
+        rc = _lib.load().frattn_layer_norm(x.data_ptr(), _stride(x), _ptr(weight), _ptr(bias), _DT[pd], T, C,
+                                           float(eps), _DT[x.dtype], out.data_ptr(), _stride(out), _ptr(mean),
+                                           _ptr(rstd), _stream(x.device))
+    _lib.check(rc, "frattn_layer_norm")
+    return (out, mean, rstd) if return_stats else out
+
+
+def layer_norm_backward(
+    dout: torch.Tensor,
+    x: torch.Tensor | PackedActivation,
+    weight: torch.Tensor | None,
+    mean: torch.Tensor,
+    rstd: torch.Tensor,
+    *,
+    param_dtype: torch.dtype | None = None,
+    need_param_grads: bool = True,
+):
+    """``(dx, dweight, dbias)`` of ``layer_norm`` for the output gradient ``dout`` ``[T, C]``.
+
+    ``x`` is the forward's input or its checkpoint, ``mean`` / ``rstd`` the forward's.
+    dweight and dbias come in ``weight``'s type (``param_dtype``, default x's, when
+    weight is None); with ``need_param_grads=False`` they are not computed (None).
+    """
+    packed = isinstance(x, PackedActivation)
+    _check_rows("dout", dout, tuple(_DT))
+    T, C = dout.shape
+    dev = dout.device
+    if packed:
+        _check_packed("x", x, dout.dtype, (T, C))
+    else:
+        _check_rows("x", x, tuple(_DT))
+        if x.shape != dout.shape or x.dtype != dout.dtype:
+            raise ValueError(f"x must match dout {tuple(dout.shape)} {dout.dtype}, got {tuple(x.shape)} {x.dtype}")
+        x = _rows(x)
+    if x.device != dev:
+        raise ValueError(f"x must be on {dev}, got {x.device}")
+    weight = None if weight is None else _check_param("weight", weight, C, dout.dtype, dev)
+    pd = weight.dtype if weight is not None else param_dtype or dout.dtype
+    if pd not in (dout.dtype, torch.float32):
+        raise ValueError(f"param_dtype must be {dout.dtype} or float32, got {pd}")
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if t.shape != (T,) or t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 [{T}] on {dev}, got {tuple(t.shape)} {t.dtype}")
+    dout = _rows(dout)
+    dx = torch.empty(T, C, dtype=dout.dtype, device=dev)
+    dw = db = ws = None
+    nbytes = 0
+    if need_param_grads:
+        dw, db = torch.empty(2, C, dtype=pd, device=dev).unbind(0)
+        with _on(dev):
+            nbytes = _lib.workspace_bytes_layer_norm_bwd(T, C)
+        ws = _workspace(nbytes, dev)
+    with _on(dev):
+        rc = _lib.load().frattn_layer_norm_bwd(
+            dout.data_ptr(), _stride(dout), None if packed else x.data_ptr(), 0 if packed else _stride(x),
+            x.codes.data_ptr() if packed else None, x.scales.data_ptr() if packed else None, _ptr(weight), _DT[pd],
+            mean.data_ptr(), rstd.data_ptr(), T, C, _DT[dout.dtype], dx.data_ptr(), C, _ptr(dw), _ptr(db), _ptr(ws),
+            nbytes, _stream(dev))
+    _lib.check(rc, "frattn_layer_norm_bwd")
+    return dx, dw, db
+
+
+class _LayerNorm(torch.autograd.Function):
+    """Autograd node of ``layer_norm``; x is kept as it is or as a checkpoint."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, checkpoint):
+        out, mean, rstd = layer_norm(x, weight, bias, eps=eps, return_stats=True)
+        ctx.has = (weight is not None, bias is not None)
+        ctx.param_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else None
+        ctx.packed = checkpoint
+        if checkpoint:
+            p = pack_activation(x)
+            ctx.meta = (p.width, p.dtype)
+            ctx.save_for_backward(p.codes, p.scales, weight, mean, rstd)
+        else:
+            ctx.save_for_backward(x, None, weight, mean, rstd)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        x, scales, weight, mean, rstd = ctx.saved_tensors
+        if ctx.packed:
+            x = PackedActivation(x, scales, *ctx.meta)
+        need = any(ctx.needs_input_grad[1:3])
+        dx, dw, db = layer_norm_backward(dout, x, weight, mean, rstd, param_dtype=ctx.param_dtype,
+                                         need_param_grads=need)
+        return dx, dw if ctx.has[0] else None, db if ctx.has[1] else None, None, None
+
+
+def layer_norm_train(x, weight=None, bias=None, *, eps: float = 1e-6, checkpoint: bool = False) -> torch.Tensor:
+    """``layer_norm`` with gradients for x, weight and bias. With ``checkpoint`` the
+    node keeps x in 8 bits, and the gradients are those at the values so kept."""
+    return _LayerNorm.apply(x, weight, bias, eps, checkpoint)
+
+
+# --------------------------------------------------------------------------- linear layer
+_LINEAR_DT = (torch.float16, torch.bfloat16)
+
+
+def _act_code(activation) -> int:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    return ACTIVATIONS[activation]
+
+
+def _check_weight(weight, K, dtype, device):
+    if weight.ndim != 2 or weight.shape[1] != K or weight.shape[0] <= 0:
+        raise ValueError(f"weight must be [N, {K}], got {tuple(weight.shape)}")
+    if weight.dtype != dtype or weight.device != device:
+        raise ValueError(f"weight must be {dtype} on {device}, got {weight.dtype} on {weight.device}")
+
+
+def linear_act(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    activation: str = "none",
+    residual: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    save_preact: str | None = None,
+):
+    """``act(x @ weight.T + bias) + residual`` in one pass, products and sums in fp32.
+
+    ``x`` ``[T, K]``, ``weight`` ``[N, K]`` (``nn.Linear`` layout), ``bias`` ``[N]``,
+    ``residual`` ``[T, N]``, all float16 or all bfloat16; ``activation`` one of
+    ``ACTIVATIONS``. ``save_preact="full"`` also returns the pre-activation
+    ``x @ weight.T + bias`` as a ``[T, N]`` tensor, ``"packed"`` as a
+    ``PackedActivation``: ``(out, preact)``. ``out`` and ``residual`` may be strided
+    rows; ``out`` may be ``residual`` itself (added in place).
+    """
+    _check_rows("x", x, _LINEAR_DT)
+    T, K = x.shape
+    dev, dt = x.device, x.dtype
+    act = _act_code(activation)
+    _check_weight(weight, K, dt, dev)
+    N = weight.shape[0]
+    if bias is not None:
+        if bias.shape != (N,) or bias.dtype != dt or bias.device != dev:
+            raise ValueError(f"bias must be [{N}] {dt} on {dev}, got {tuple(bias.shape)} {bias.dtype} on {bias.device}")
+        bias = bias.contiguous()
+    if residual is not None:
+        if residual.shape != (T, N) or residual.dtype != dt or residual.device != dev:
+            raise ValueError(f"residual must be [{T}, {N}] {dt} on {dev}, got {tuple(residual.shape)} "
+                             f"{residual.dtype} on {residual.device}")
+        residual = _rows(residual)
+    if save_preact not in (None, "none", "full", "packed"):
+        raise ValueError(f"save_preact must be None, 'full' or 'packed', got {save_preact!r}")
+    out = _check_out_rows(out, (T, N), x)
+    z = p = None
+    if save_preact == "full":
+        z = torch.empty(T, N, dtype=dt, device=dev)
+    elif save_preact == "packed":
+        p = _empty_packed(T, N, dt, dev)
+    if T > 0:
+        x, weight = _rows16(x), _rows16(weight)
+        with _on(dev):
+            nbytes = _lib.workspace_bytes_linear_act(T, K, N)
+            ws = _workspace(nbytes, dev) if nbytes else None
+            rc = _lib.load().frattn_linear_act(
+                x.data_ptr(), _row16_stride(x), weight.data_ptr(), _row16_stride(weight), _ptr(bias), _ptr(residual),
+                0 if residual is None else _stride(residual), act, T, K, N, _DT[dt], out.data_ptr(), _stride(out),
+                _ptr(z), N, p.codes.data_ptr() if p is not None else None,
+                p.scales.data_ptr() if p is not None else None, _ptr(ws), nbytes, _status_word(dev).data_ptr(),
+                _stream(dev))
+        _lib.check(rc, "frattn_linear_act")
+    if save_preact in (None, "none"):
+        return out
+    return out, (z if p is None else p)
+
+
+def _row16_stride(t: torch.Tensor) -> int:
+    """Row stride of a ``_rows16`` matrix (of a single row: any valid one)."""
+    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
+
+
+def linear_act_backward(
+    dout: torch.Tensor,
+    x: torch.Tensor | PackedActivation,
+    weight: torch.Tensor,
+    preact: torch.Tensor | PackedActivation | None = None,
+    *,
+    activation: str = "none",
+    need: tuple[bool, bool, bool] = (True, True, True),
+):
+    """``(dx, dweight, dbias)`` of ``linear_act`` for the output gradient ``dout`` ``[T, N]``.
+
+    With ``dz = dout * act'(preact)``: ``dx = dz @ weight``, ``dweight = dz.T @ x``,
+    ``dbias = dz.sum(0)``, in x's type. ``x`` and ``preact`` (what ``save_preact``
+    returned; unused for activation "none") may be checkpoints. ``need`` says which
+    of the three are wanted; the others come as None. The residual's gradient is
+    ``dout``.
+    """
+    _check_rows("dout", dout, _LINEAR_DT)
+    T, N = dout.shape
+    dev, dt = dout.device, dout.dtype
+    act = _act_code(activation)
+    if weight.ndim != 2 or weight.shape[0] != N or weight.shape[1] <= 0:
+        raise ValueError(f"weight must be [{N}, K], got {tuple(weight.shape)}")
+    K = weight.shape[1]
+    _check_weight(weight, K, dt, dev)
+    xp, zp = isinstance(x, PackedActivation), isinstance(preact, PackedActivation)
+    if xp:
+        _check_packed("x", x, dt, (T, K))
+    else:
+        _check_rows("x", x, _LINEAR_DT)
+        if x.shape != (T, K) or x.dtype != dt:
+            raise ValueError(f"x must be [{T}, {K}] {dt}, got {tuple(x.shape)} {x.dtype}")
+    if x.device != dev:
+        raise ValueError(f"x must be on {dev}, got {x.device}")
+    if act:
+        if preact is None:
+            raise ValueError(f"preact is needed for activation {activation!r}")
+        if zp:
+            _check_packed("preact", preact, dt, (T, N))
+        else:
+            _check_rows("preact", preact, _LINEAR_DT)
+            if preact.shape != (T, N) or preact.dtype != dt:
+                raise ValueError(f"preact must be [{T}, {N}] {dt}, got {tuple(preact.shape)} {preact.dtype}")
+            preact = _rows(preact)
+        if preact.device != dev:
+            raise ValueError(f"preact must be on {dev}, got {preact.device}")
+    else:
+        preact, zp = None, False
+    dout = _rows(dout)
+    need_x, need_w, need_b = need
+    dx = torch.empty(T, K, dtype=dt, device=dev) if need_x else None
+    dw = torch.empty(N, K, dtype=dt, device=dev) if need_w else None
+    db = torch.empty(N, dtype=dt, device=dev) if need_b else None
+    if not (need_x or need_w or need_b):
+        return dx, dw, db
+    if not xp and need_w:
+        x = _rows16(x)
+    if need_x:
+        weight = _rows16(weight)
+    with _on(dev):
+        nbytes = _lib.workspace_bytes_linear_act_bwd(T, K, N)
+        ws = _workspace(nbytes, dev)
+        rc = _lib.load().frattn_linear_act_bwd(
+            dout.data_ptr(), _stride(dout), None if xp else x.data_ptr(), 0 if xp else _row16_stride(x),
+            x.codes.data_ptr() if xp else None, x.scales.data_ptr() if xp else None, weight.data_ptr(),
+            _row16_stride(weight), None if preact is None or zp else preact.data_ptr(),
+            0 if preact is None or zp else _stride(preact), preact.codes.data_ptr() if zp else None,
+            preact.scales.data_ptr() if zp else None, act, T, K, N, _DT[dt], _ptr(dx), K, _ptr(dw), _ptr(db),
+            ws.data_ptr(), nbytes, _status_word(dev).data_ptr(), _stream(dev))
+    _lib.check(rc, "frattn_linear_act_bwd")
+    return dx, dw, db
+
+
+class _LinearAct(torch.autograd.Function):
+    """Autograd node of ``linear_act``; x and the pre-activation are kept as they are
+    or as checkpoints."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, checkpoint):
+        save = None if activation == "none" else "packed" if checkpoint else "full"
+        got = linear_act(x, weight, bias, activation=activation, residual=residual, save_preact=save)
+        out, z = got if save else (got, None)
+        ctx.activation, ctx.packed = activation, checkpoint
+        ctx.has_bias, ctx.has_res = bias is not None, residual is not None
+        if checkpoint:
+            p = pack_activation(x)
+            ctx.meta = (p.width, z.width if z is not None else 0, x.dtype)
+            ctx.save_for_backward(weight, p.codes, p.scales, *((z.codes, z.scales) if z is not None else ()))
+        else:
+            ctx.save_for_backward(weight, x, *((z,) if z is not None else ()))
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        weight, *kept = ctx.saved_tensors
+        if ctx.packed:
+            kx, kz, dt = ctx.meta
+            x = PackedActivation(kept[0], kept[1], kx, dt)
+            z = PackedActivation(kept[2], kept[3], kz, dt) if kz else None
+        else:
+            x, z = kept[0], kept[1] if len(kept) > 1 else None
+        need = ctx.needs_input_grad
+        dx, dw, db = linear_act_backward(dout, x, weight, z, activation=ctx.activation,
+                                         need=(need[0], need[1], ctx.has_bias and need[2]))
+        return dx, dw, db, dout if ctx.has_res and need[3] else None, None, None
+
+
+def linear_act_train(x, weight, bias=None, *, activation: str = "none", residual=None,
+                     checkpoint: bool = False) -> torch.Tensor:
+    """``linear_act`` with gradients for x, weight, bias and residual. With
+    ``checkpoint`` the node keeps x and the pre-activation in 8 bits, and the
+    gradients are those at the values so kept."""
+    return _LinearAct.apply(x, weight, bias, residual, activation, checkpoint)

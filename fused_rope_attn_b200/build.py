@@ -25,7 +25,10 @@ WINDOW_SRC = os.path.join(CSRC, "frattn_window.cu")
 QKV_SRC = os.path.join(CSRC, "frattn_qkv.cu")
 BWD_SRC = os.path.join(CSRC, "frattn_bwd.cu")
 FP8_SRC = os.path.join(CSRC, "frattn_fp8.cu")
-DEPS = [HOST_SRC, INST_SRC, WINDOW_SRC, QKV_SRC, BWD_SRC, FP8_SRC, os.path.join(CSRC, "frattn_kernel.cuh"), os.path.join(CSRC, "frattn_ptx.cuh"),
+NORM_SRC = os.path.join(CSRC, "frattn_norm.cu")
+LINEAR_SRC = os.path.join(CSRC, "frattn_linear.cu")
+DEPS = [HOST_SRC, INST_SRC, WINDOW_SRC, QKV_SRC, BWD_SRC, FP8_SRC, NORM_SRC, LINEAR_SRC, os.path.join(CSRC, "frattn_kernel.cuh"),
+        os.path.join(CSRC, "frattn_ptx.cuh"), os.path.join(CSRC, "frattn_block.cuh"),
         os.path.join(ROOT, "include", "frattn.h")]
 OUT = os.path.join(HERE, "libfrattn.so")
 OBJ_DIR = os.path.join(HERE, "_build")
@@ -83,6 +86,10 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
     qkv_obj = os.path.join(OBJ_DIR, "frattn_qkv.o")
     cmds.append([nvcc(), *NVCC_FLAGS, *extra, "-c", "-o", qkv_obj, QKV_SRC])
     objs.append(qkv_obj)
+    for name, src in (("frattn_norm.o", NORM_SRC), ("frattn_linear.o", LINEAR_SRC)):
+        obj = os.path.join(OBJ_DIR, name)
+        cmds.append([nvcc(), *NVCC_FLAGS, *extra, "-c", "-o", obj, src])
+        objs.append(obj)
     host_obj = os.path.join(OBJ_DIR, "frattn_host.o")
     cmds.append([nvcc(), *NVCC_FLAGS, *extra, "-c", "-o", host_obj, HOST_SRC])
     objs.append(host_obj)

@@ -1,0 +1,178 @@
+// Device helpers shared by the transformer-block operators (layer norm, linear
+// layer with epilogue, 8-bit activation checkpoints): vector access to rows of
+// any alignment, the checkpoint format, and the activations with derivatives.
+#pragma once
+#include "frattn_kernel.cuh"
+
+namespace frattn {
+
+// ---------------------------------------------------------------- rows as vectors
+// VEC consecutive elements of a row. A kernel instance for VEC is launched only
+// when every row start is aligned to min(16, VEC * sizeof(T)) bytes and VEC
+// divides the row length (row_vec below), so no access leaves its row.
+template <typename T>
+__device__ __forceinline__ float elem_f32(T x);
+template <>
+__device__ __forceinline__ float elem_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float elem_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float elem_f32<__half>(__half x) { return __half2float(x); }
+
+template <typename T>
+__device__ __forceinline__ T f32_elem(float x);
+template <>
+__device__ __forceinline__ float f32_elem<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 f32_elem<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half f32_elem<__half>(float x) { return __float2half_rn(x); }
+
+template <int BYTES>
+struct RawVec;
+template <>
+struct RawVec<2> { using type = uint16_t; };
+template <>
+struct RawVec<4> { using type = uint32_t; };
+template <>
+struct RawVec<8> { using type = uint2; };
+template <>
+struct RawVec<16> { using type = uint4; };
+
+// VEC elements as raw words (loads of several vectors can be in flight before
+// any of them is converted).
+template <typename T, int VEC>
+struct Vec {
+  static constexpr int kBytes = VEC * static_cast<int>(sizeof(T));
+  static constexpr int kPart = kBytes > 16 ? 16 : kBytes;
+  static constexpr int kParts = kBytes / kPart;
+  using Raw = typename RawVec<kPart>::type;
+  union {
+    Raw raw[kParts];
+    T elem[VEC];
+  };
+  __device__ __forceinline__ Vec() {}
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) raw[i] = __ldg(reinterpret_cast<const Raw*>(p) + i);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) reinterpret_cast<Raw*>(p)[i] = raw[i];
+  }
+  __device__ __forceinline__ float get(int i) const { return elem_f32<T>(elem[i]); }
+  __device__ __forceinline__ void set(int i, float x) { elem[i] = f32_elem<T>(x); }
+};
+
+// Largest vector width of {8, 4, 1} elements of esz bytes that every listed
+// pointer and row stride (elements) allows for rows of C elements.
+struct RowVec {
+  int C, esz;
+  int v = 8;
+  RowVec(int C_, int esz_) : C(C_), esz(esz_) {
+    while (v > 1 && C % v) v = v == 8 ? 4 : 1;
+  }
+  RowVec& row(const void* p, long long stride, int e = 0) {
+    if (!p) return *this;
+    const int es = e ? e : esz;
+    auto ok = [&](int w) {
+      const int a = w * es < 16 ? w * es : 16;
+      return reinterpret_cast<uintptr_t>(p) % a == 0 && (stride * es) % a == 0;
+    };
+    while (v > 1 && !ok(v)) v = v == 8 ? 4 : 1;
+    return *this;
+  }
+};
+
+inline bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// ---------------------------------------------------------------- 8-bit checkpoints
+// A row of C values in blocks of 32: codes [T, 32 nb] int8, scale bytes [T, nb],
+// nb = ceil(C / 32). With amax = f 2^q, 1/2 <= f < 1, the block's largest
+// magnitude: e = max(q - 7, -126), scale byte e + 127, code = rint(x / 2^e)
+// limited to [-127, 127]. A power-of-two scale makes both directions exact but
+// for that one rounding: x 2^-e is exact in 32 bits, and code 2^e has 7
+// significant bits, so it is exact in bf16 and fp32 (and, for values that came
+// from fp16, in fp16): a gradient computed from a checkpoint rounds it no
+// further. A block that holds an infinity or a NaN gets scale byte 255 and
+// stands for NaN throughout, so that it is not lost.
+constexpr int kPackBlock = 32;
+constexpr uint32_t kPackNan = 255;
+
+__host__ __device__ inline long long pack_blocks(int C) { return (static_cast<long long>(C) + kPackBlock - 1) / kPackBlock; }
+
+// Scale byte of a block from the largest (x as bits) & 0x7fffffff of its values
+// (integer order of the magnitudes; NaNs come out on top).
+__device__ __forceinline__ uint32_t pack_scale(uint32_t amax_bits) {
+  const uint32_t e = amax_bits >> 23;  // q + 126
+  return e == 255u ? kPackNan : (e > 7u ? e : 7u) - 6u;
+}
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// 2^-e of a scale byte; 0 for a NaN block (whose codes are then 0).
+__device__ __forceinline__ float pack_inv(uint32_t scale) {
+  return scale == kPackNan ? 0.f : __uint_as_float((254u - scale) << 23);
+}
+// 2^e of a scale byte; NaN for a NaN block.
+__device__ __forceinline__ float pack_step(uint32_t scale) {
+  return scale == kPackNan ? __uint_as_float(0x7fffffffu) : __uint_as_float(scale << 23);
+}
+__device__ __forceinline__ int pack_code(float x, float inv) {
+  const float t = x * inv;
+  // (inv = 0 with x infinite or NaN: the comparison is false, the code 0)
+  const float c = fabsf(t) <= 127.f ? t : (t > 127.f ? 127.f : (t < -127.f ? -127.f : 0.f));
+  return __float2int_rn(c);
+}
+
+// ---------------------------------------------------------------- activations
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / (1 + e^-z): relative error of a few 2^-23 (the two approximations' own);
+// 0 and 1 at the ends.
+__device__ __forceinline__ float sigmoid_f(float z) { return rcp_fast(1.f + exp2_fast(-1.4426950408889634f * z)); }
+
+// Standard normal distribution function, (1 + erf(z / sqrt 2)) / 2.
+__device__ __forceinline__ float normal_cdf(float z) { return 0.5f + 0.5f * erff(z * 0.70710678118654752f); }
+
+template <int ACT>
+__device__ __forceinline__ float act_f(float z) {
+  if constexpr (ACT == FRATTN_ACT_RELU) {
+    return z > 0.f ? z : (z != z ? z : 0.f);
+  } else if constexpr (ACT == FRATTN_ACT_GELU) {
+    return z * normal_cdf(z);
+  } else if constexpr (ACT == FRATTN_ACT_GELU_TANH) {
+    // z (1 + tanh u) / 2 = z / (1 + e^-2u), u = sqrt(2 / pi) (z + 0.044715 z^3)
+    return z * sigmoid_f(1.5957691216057308f * z * (1.f + 0.044715f * z * z));
+  } else if constexpr (ACT == FRATTN_ACT_SILU) {
+    return z * sigmoid_f(z);
+  } else {
+    return z;
+  }
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_grad_f(float z) {
+  if constexpr (ACT == FRATTN_ACT_RELU) {
+    return z > 0.f ? 1.f : (z != z ? z : 0.f);
+  } else if constexpr (ACT == FRATTN_ACT_GELU) {
+    return normal_cdf(z) + z * 0.3989422804014327f * exp2_fast(-0.7213475204444817f * z * z);
+  } else if constexpr (ACT == FRATTN_ACT_GELU_TANH) {
+    const float s = sigmoid_f(1.5957691216057308f * z * (1.f + 0.044715f * z * z));
+    const float zc = fminf(fmaxf(z, -64.f), 64.f);  // s (1 - s) is 0 beyond: keeps 0 x infinity out
+    return z != z ? z : s + zc * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * zc * zc);
+  } else if constexpr (ACT == FRATTN_ACT_SILU) {
+    const float s = sigmoid_f(z);
+    return s + s * (1.f - s) * z;
+  } else {
+    return 1.f;
+  }
+}
+
+}  // namespace frattn

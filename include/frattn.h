@@ -251,6 +251,83 @@ int frattn_fwd_noalloc(const void* q, const void* k, const void* v, const void* 
                        int H, int D, int max_seqlen, int in_dtype, void* out, int32_t* status,
                        void* stream);
 
+/* ---- Transformer block around the attention (the reference has the attention
+ * alone; its caller's block is library calls): layer norm, linear layer with
+ * bias, activation and residual in its epilogue, each with its backward pass, and
+ * activation checkpoints in 8 bits. Matrices are rows of a row stride given in
+ * elements; sums are kept in fp32 and rounded once to the output's type.
+ *
+ * Checkpoints: a row of C values in nb = ceil(C / 32) blocks of 32, as codes
+ * [T, 32 nb] int8 (contiguous, 16-byte aligned; zeros past C) and scale bytes
+ * [T, nb]. With amax = f 2^q (1/2 <= f < 1) the largest magnitude of a block,
+ * e = max(q - 7, -126): scale byte e + 127, code = rint(x / 2^e) limited to
+ * [-127, 127], value code 2^e (exact in bf16 and fp32). A block holding an
+ * infinity or a NaN has scale byte 255 and stands for NaN throughout.
+ *
+ * frattn_act_pack / frattn_act_unpack: x [T, C] (F32, F16 or BF16) to a
+ * checkpoint, and back to out [T, C] of any of these types.
+ *
+ * frattn_layer_norm: out = (x - mean) rstd weight + bias per row of C values,
+ * mean = sum x / C, rstd = 1 / sqrt(sum (x - mean)^2 / C + eps).
+ *   x, out       : [T, C], dtype F32, F16 or BF16
+ *   weight, bias : [C] of param_dtype (dtype or F32), or NULL (ones / zeros)
+ *   mean, rstd   : [T] fp32 or NULL
+ * frattn_layer_norm_bwd: with h = (x - mean) rstd and g = dout weight,
+ *   dx = rstd (g - mean(g) - h mean(g h)), dweight = sum_rows dout h,
+ *   dbias = sum_rows dout (either may be NULL); x as [T, C] or as a checkpoint
+ *   (x NULL, codes and scales given). The sums over rows are added in a fixed
+ *   order. workspace >= frattn_workspace_bytes_layer_norm_bwd(T, C), 16-byte aligned. */
+int frattn_act_pack(const void* x, long long x_stride, int T, int C, int dtype, int8_t* codes,
+                    uint8_t* scales, void* stream);
+int frattn_act_unpack(const int8_t* codes, const uint8_t* scales, int T, int C, int dtype, void* out,
+                      long long out_stride, void* stream);
+int frattn_layer_norm(const void* x, long long x_stride, const void* weight, const void* bias,
+                      int param_dtype, int T, int C, float eps, int dtype, void* out,
+                      long long out_stride, float* mean, float* rstd, void* stream);
+int frattn_workspace_bytes_layer_norm_bwd(int T, int C, size_t* bytes);
+int frattn_layer_norm_bwd(const void* dout, long long dout_stride, const void* x, long long x_stride,
+                          const int8_t* codes, const uint8_t* scales, const void* weight,
+                          int param_dtype, const float* mean, const float* rstd, int T, int C,
+                          int dtype, void* dx, long long dx_stride, void* dweight, void* dbias,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Activations of the linear layer. */
+enum {
+  FRATTN_ACT_NONE = 0,
+  FRATTN_ACT_RELU = 1,
+  FRATTN_ACT_GELU = 2,      /* z (1 + erf(z / sqrt 2)) / 2 */
+  FRATTN_ACT_GELU_TANH = 3, /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+  FRATTN_ACT_SILU = 4       /* z / (1 + e^-z) */
+};
+
+/* frattn_linear_act: z = x W^T + bias, out = act(z) + residual.
+ *   x : [T, K], w : [N, K] (nn.Linear layout), both F16 or BF16 (dtype) with
+ *       16-byte aligned rows (strides multiples of 8; FRATTN_E_ALIGN otherwise)
+ *   bias : [N] or NULL, residual : [T, N] or NULL, out : [T, N], of dtype
+ *   z : [T, N] of dtype, or z_codes / z_scales (a checkpoint of z), or all NULL:
+ *       where the pre-activation the backward pass needs is written
+ * z is summed in fp32; act and residual are applied to the fp32 value.
+ * frattn_linear_act_bwd: with dz = dout act'(z),
+ *   dx = dz W [T, K], dw = dz^T x [N, K], db = sum_rows dz [N] (each may be NULL),
+ *   x and z as matrices or as checkpoints (z unused for FRATTN_ACT_NONE). The
+ *   residual's gradient is dout itself. dz is rounded to dtype once, as the
+ *   operand of the two products; db is summed before that rounding. x, w: rows
+ *   16-byte aligned as above. Sums over rows are added in a fixed order.
+ * Workspaces: at least the bytes the queries give, 256-byte aligned. */
+int frattn_workspace_bytes_linear_act(int T, int K, int N, size_t* bytes);
+int frattn_linear_act(const void* x, long long x_stride, const void* w, long long w_stride,
+                      const void* bias, const void* residual, long long res_stride, int activation,
+                      int T, int K, int N, int dtype, void* out, long long out_stride, void* z,
+                      long long z_stride, int8_t* z_codes, uint8_t* z_scales, void* workspace,
+                      size_t workspace_bytes, int32_t* status, void* stream);
+int frattn_workspace_bytes_linear_act_bwd(int T, int K, int N, size_t* bytes);
+int frattn_linear_act_bwd(const void* dout, long long dout_stride, const void* x, long long x_stride,
+                          const int8_t* x_codes, const uint8_t* x_scales, const void* w,
+                          long long w_stride, const void* z, long long z_stride,
+                          const int8_t* z_codes, const uint8_t* z_scales, int activation, int T,
+                          int K, int N, int dtype, void* dx, long long dx_stride, void* dw, void* db,
+                          void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
 /* ---- Window plan on the device (no host-side index arithmetic, no large
  * host->device copies). Replaces the host producers of the kernel's inputs:
  *   utils.py:12-102        get_window_index(grid_thw, window_size, merge, patch)
