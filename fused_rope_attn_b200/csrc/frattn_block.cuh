@@ -116,11 +116,20 @@ __device__ __forceinline__ float pack_inv(uint32_t scale) {
 __device__ __forceinline__ float pack_step(uint32_t scale) {
   return scale == kPackNan ? __uint_as_float(0x7fffffffu) : __uint_as_float(scale << 23);
 }
-__device__ __forceinline__ int pack_code(float x, float inv) {
-  const float t = x * inv;
-  // (inv = 0 with x infinite or NaN: the comparison is false, the code 0)
-  const float c = fabsf(t) <= 127.f ? t : (t > 127.f ? 127.f : (t < -127.f ? -127.f : 0.f));
-  return __float2int_rn(c);
+// Largest magnitude that a code of the block stands for; 0 for a NaN block, whose
+// codes are 0.
+__device__ __forceinline__ float pack_limit(uint32_t scale) {
+  return scale == kPackNan ? 0.f : 127.f * __uint_as_float(scale << 23);
+}
+// Code of x in the low byte: x / 2^e is exact, and adding 1.5 2^23 rounds it to the
+// nearest integer (ties to even) in two's complement.
+__device__ __forceinline__ uint32_t pack_code(float x, float inv, float lim) {
+  return __float_as_uint(fmaf(fminf(fmaxf(x, -lim), lim), inv, 12582912.f));
+}
+__device__ __forceinline__ uint32_t pack_code4(float a, float b, float c, float d, float inv, float lim) {
+  const uint32_t lo = __byte_perm(pack_code(a, inv, lim), pack_code(b, inv, lim), 0x0040);
+  const uint32_t hi = __byte_perm(pack_code(c, inv, lim), pack_code(d, inv, lim), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
 }
 
 // ---------------------------------------------------------------- activations
@@ -138,15 +147,29 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // 0 and 1 at the ends.
 __device__ __forceinline__ float sigmoid_f(float z) { return rcp_fast(1.f + exp2_fast(-1.4426950408889634f * z)); }
 
-// Standard normal distribution function, (1 + erf(z / sqrt 2)) / 2.
-__device__ __forceinline__ float normal_cdf(float z) { return 0.5f + 0.5f * erff(z * 0.70710678118654752f); }
+// Standard normal distribution function and e^(-z^2 / 2) (also a factor of its
+// density): Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26, with
+// x = |z| / sqrt 2: erf x = 1 - (a1 t + ... + a5 t^5) e^-x^2 + d, |d| < 1.5e-7,
+// t = 1 / (1 + p x). Half of that in the distribution function, far below the
+// rounding of a 16-bit result; a third of erff's instructions and no branch.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float t = rcp_fast(fmaf(fabsf(z), 0.23164191f, 1.f));  // p / sqrt 2
+  e = exp2_fast(-0.7213475204444817f * z * z);
+  float q = fmaf(t, 0.5307027145f, -0.7265760135f);  // halves of a5 ... a1
+  q = fmaf(q, t, 0.7107068705f);
+  q = fmaf(q, t, -0.142248368f);
+  q = fmaf(q, t, 0.127414796f);
+  q = q * t * e;
+  return z < 0.f ? q : 1.f - q;
+}
 
 template <int ACT>
 __device__ __forceinline__ float act_f(float z) {
   if constexpr (ACT == FRATTN_ACT_RELU) {
     return z > 0.f ? z : (z != z ? z : 0.f);
   } else if constexpr (ACT == FRATTN_ACT_GELU) {
-    return z * normal_cdf(z);
+    float e;
+    return z * normal_cdf(z, e);
   } else if constexpr (ACT == FRATTN_ACT_GELU_TANH) {
     // z (1 + tanh u) / 2 = z / (1 + e^-2u), u = sqrt(2 / pi) (z + 0.044715 z^3)
     return z * sigmoid_f(1.5957691216057308f * z * (1.f + 0.044715f * z * z));
@@ -162,7 +185,9 @@ __device__ __forceinline__ float act_grad_f(float z) {
   if constexpr (ACT == FRATTN_ACT_RELU) {
     return z > 0.f ? 1.f : (z != z ? z : 0.f);
   } else if constexpr (ACT == FRATTN_ACT_GELU) {
-    return normal_cdf(z) + z * 0.3989422804014327f * exp2_fast(-0.7213475204444817f * z * z);
+    float e;
+    const float c = normal_cdf(z, e);
+    return fmaf(z * e, 0.3989422804014327f, c);
   } else if constexpr (ACT == FRATTN_ACT_GELU_TANH) {
     const float s = sigmoid_f(1.5957691216057308f * z * (1.f + 0.044715f * z * z));
     const float zc = fminf(fmaxf(z, -64.f), 64.f);  // s (1 - s) is 0 beyond: keeps 0 x infinity out

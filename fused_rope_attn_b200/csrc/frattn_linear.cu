@@ -13,109 +13,684 @@ int column_finish(const float* partial, int groups, int arrays, int C, void* out
 int act_unpack(const int8_t* codes, const uint8_t* scales, int T, int C, int dtype, void* out, long long out_stride,
                cudaStream_t st);
 
-// D[m, n] = sum_k A[m, k] B[n, k] with element strides, then the epilogue.
-struct MatmulParams {
-  const void *a, *b;
-  long long a_m, a_k, b_n, b_k;
-  int M, N, K;
-  const void* bias;  // [N] or null
-  const void* res;   // [M, N] or null
+// One product D[m, n] = sum_k A[m, k] B[n, k] and its epilogue. A and B are matrices of
+// 16-bit rows; an operand is "K-major" when its rows run along k (x and W in the
+// forward product), "MN-major" when they run along m or n (W in dz W, both in dz^T x).
+struct GemmParams {
+  CUtensorMap tma_a, tma_b;
+  CUtensorMap tma_out, tma_z;  // box {64, 32}, 128-byte swizzle; used where out_tma / z_tma
+  const void* bias;            // [N] or null
+  const void* res;             // [M, N] or null
   long long res_stride;
   int act;
   void* out;
   long long out_stride;
-  void* z;
+  void* z;  // or null
   long long z_stride;
-  int8_t* z_codes;
+  int8_t* z_codes;  // or null
   uint8_t* z_scales;
+  int out_tma, z_tma;          // written by TMA stores (16-byte rows), else element stores of
+  int out_w, z_w;              // 4, 2 or 1 elements
+  int res_vec;                 // residual rows are 16-byte aligned
+  int M, N, nk;                // nk: 64-wide steps of the reduction
+  int tiles_n, tiles;
+  int split;                   // 0: a pair owns whole tiles; else k steps per pair (see Segments)
+  float* partial;              // [2 pairs][256][BN] (split)
+  int32_t* status;
+  unsigned long long wait_limit_ns;
 };
 
 namespace {
 
-__device__ __forceinline__ float act_any(int act, float z) {
+constexpr int kGemmThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
+constexpr int kGemmEpiWarps = 8;
+
+template <int BN>
+struct GemmCfg {
+  static constexpr int BK = 64;
+  static constexpr int A_BYTES = 128 * BK * 2;
+  static constexpr int B_BYTES = BN / 2 * BK * 2;
+  static constexpr int STAGE = A_BYTES + B_BYTES;
+  static constexpr int CHUNKS = BN / 128;           // 64-column chunks per epilogue warp and tile
+  static constexpr int STG = 32 * 64 * 2;           // one warp's 32 x 64 output chunk
+  static constexpr int STG_BYTES = kGemmEpiWarps * 2 * STG;
+  static constexpr int BIAS_BYTES = kGemmEpiWarps * 64 * 4;
+  static constexpr int ST_FIT = (227 * 1024 - 1024 - 512 - STG_BYTES - BIAS_BYTES) / STAGE;
+  static constexpr int ST = ST_FIT > 8 ? 8 : ST_FIT;
+  static constexpr int OFF_STG = ST * STAGE;
+  static constexpr int OFF_BIAS = OFF_STG + STG_BYTES;
+  static constexpr int OFF_BAR = OFF_BIAS + BIAS_BYTES;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;  // barriers + 1024-B alignment slack
+  static_assert(STAGE % 1024 == 0 && OFF_STG % 1024 == 0, "128-B swizzle atoms");
+  static_assert((2 * ST + 5) * 8 + 8 <= 256, "barriers");
+};
+
+// The tiles (or parts of tiles) a CTA pair computes, in order; every role of the
+// kernel walks the same list.
+//  * whole tiles: t = pair, pair + pairs, ... with all nk steps each;
+//  * split: the nk steps of all tiles, laid end to end, are dealt out in equal runs
+//    of `split` steps. A pair's run covers at most one part at the end of a tile
+//    that an earlier pair began, whole tiles, and one part at the beginning of a
+//    tile that it does not finish. Parts go to the pair's two partial slots as
+//    fp32 sums; gemm_finish_kernel adds a tile's parts in the order of k.
+struct Segments {
+  int t, k0, k1;
+  int pos, end, step, split, nk, tiles;
+  __device__ __forceinline__ Segments(const GemmParams& p, int pair, int pairs) {
+    split = p.split;
+    nk = p.nk;
+    tiles = p.tiles;
+    if (split) {
+      const long long total = static_cast<long long>(tiles) * nk;
+      const long long b = static_cast<long long>(pair) * split;
+      pos = static_cast<int>(b < total ? b : total);
+      end = static_cast<int>(b + split < total ? b + split : total);
+      step = 0;
+    } else {
+      pos = pair;
+      end = tiles;
+      step = pairs;
+    }
+  }
+  __device__ __forceinline__ bool next() {
+    if (pos >= end) return false;
+    if (split) {
+      t = pos / nk;
+      k0 = pos - t * nk;
+      const int room = end - pos;
+      k1 = nk - k0 < room ? nk : k0 + room;
+      pos += k1 - k0;
+    } else {
+      t = pos;
+      k0 = 0;
+      k1 = nk;
+      pos += step;
+    }
+    return true;
+  }
+  __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == nk; }
+};
+
+__device__ __forceinline__ bool gemm_wait(uint32_t bar, uint32_t parity, const GemmParams& p,
+                                          volatile int* abort_flag, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  uint32_t n = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    if ((++n & 15u) == 0) {
+      if (*abort_flag) return false;
+      if (globaltimer_ns() - t0 > p.wait_limit_ns) {
+        *abort_flag = 1;
+        if (p.status) atomicCAS(reinterpret_cast<int*>(p.status), 0, code);
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
+// Drain wait used while unwinding: ignores the abort flag, gives up after limit.
+__device__ __forceinline__ void gemm_drain(uint32_t bar, uint32_t parity, unsigned long long limit) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - t0 > limit) return;
+}
+
+template <int ACT, int N>
+__device__ __forceinline__ void act_all(float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = act_f<ACT>(v[i]);
+}
+template <int N>
+__device__ __forceinline__ void act_any(int act, float (&v)[N]) {
   switch (act) {
-    case FRATTN_ACT_RELU: return act_f<FRATTN_ACT_RELU>(z);
-    case FRATTN_ACT_GELU: return act_f<FRATTN_ACT_GELU>(z);
-    case FRATTN_ACT_GELU_TANH: return act_f<FRATTN_ACT_GELU_TANH>(z);
-    case FRATTN_ACT_SILU: return act_f<FRATTN_ACT_SILU>(z);
-    default: return z;
+    case FRATTN_ACT_RELU: return act_all<FRATTN_ACT_RELU>(v);
+    case FRATTN_ACT_GELU: return act_all<FRATTN_ACT_GELU>(v);
+    case FRATTN_ACT_GELU_TANH: return act_all<FRATTN_ACT_GELU_TANH>(v);
+    case FRATTN_ACT_SILU: return act_all<FRATTN_ACT_SILU>(v);
+    default: return;
   }
 }
 
-// 64 x 64 tile of D per block of 256 threads, 4 x 4 values per thread, fp32 FMAs.
+// 32 values of row r into columns [32 half, 32 half + 32) of a warp's [32][64] 16-bit
+// staging chunk (rows of 128 bytes, 128-byte swizzle: 16-byte piece c of row r lies at
+// c ^ (r & 7), which is what the TMA store expects and spreads the lanes over the banks).
 template <typename T>
-__global__ void __launch_bounds__(256) matmul_kernel(const MatmulParams p) {
-  __shared__ float as[16][65], bs[16][65];
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += 16) {
-    for (int i = threadIdx.x; i < 1024; i += 256) {
-      const int k = p.a_k == 1 ? i & 15 : i >> 6, m = p.a_k == 1 ? i >> 4 : i & 63;
-      as[k][m] = m0 + m < p.M && k0 + k < p.K
-                     ? elem_f32<T>(static_cast<const T*>(p.a)[(m0 + m) * p.a_m + (k0 + k) * p.a_k]) : 0.f;
-      const int kb = p.b_k == 1 ? i & 15 : i >> 6, n = p.b_k == 1 ? i >> 4 : i & 63;
-      bs[kb][n] = n0 + n < p.N && k0 + kb < p.K
-                      ? elem_f32<T>(static_cast<const T*>(p.b)[(n0 + n) * p.b_n + (k0 + kb) * p.b_k]) : 0.f;
-    }
-    __syncthreads();
+__device__ __forceinline__ void stage32(uint8_t* stg, int r, int half, const float (&v)[32]) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      float a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = as[k][ty * 4 + i];
-        b[i] = bs[k][tx * 4 + i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += a[i] * b[j];
-    }
-    __syncthreads();
-  }
-  const int nb = static_cast<int>(pack_blocks(p.N));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long m = m0 + ty * 4 + i;
-    uint32_t amax = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx * 4 + j;
-      if (n < p.N && p.bias) acc[i][j] += elem_f32<T>(static_cast<const T*>(p.bias)[n]);
-      if (n < p.N) amax = max(amax, abs_bits(acc[i][j]));
-    }
-    if (p.z_codes) {  // 8 neighbouring threads hold a block of 32 columns
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      const uint32_t scale = pack_scale(amax);
-      const float inv = pack_inv(scale);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = n0 + tx * 4 + j;
-        if (m < p.M && n < nb * kPackBlock)
-          p.z_codes[m * nb * kPackBlock + n] = n < p.N ? static_cast<int8_t>(pack_code(acc[i][j], inv)) : 0;
-      }
-      if (m < p.M && (tx & 7) == 0 && n0 + tx * 4 < p.N)
-        p.z_scales[m * nb + (n0 + tx * 4) / kPackBlock] = static_cast<uint8_t>(scale);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx * 4 + j;
-      if (m >= p.M || n >= p.N) continue;
-      if (p.z) static_cast<T*>(p.z)[m * p.z_stride + n] = f32_elem<T>(acc[i][j]);
-      float y = act_any(p.act, acc[i][j]);
-      if (p.res) y += elem_f32<T>(static_cast<const T*>(p.res)[m * p.res_stride + n]);
-      static_cast<T*>(p.out)[m * p.out_stride + n] = f32_elem<T>(y);
-    }
+  for (int c = 0; c < 4; ++c) {
+    uint4 w;
+    w.x = pack2<T>(v[8 * c + 0], v[8 * c + 1]);
+    w.y = pack2<T>(v[8 * c + 2], v[8 * c + 3]);
+    w.z = pack2<T>(v[8 * c + 4], v[8 * c + 5]);
+    w.w = pack2<T>(v[8 * c + 6], v[8 * c + 7]);
+    *reinterpret_cast<uint4*>(stg + r * 128 + (((4 * half + c) ^ (r & 7)) << 4)) = w;
   }
 }
 
-template <typename T>
-int matmul(const MatmulParams& p, cudaStream_t st) {
-  matmul_kernel<T><<<dim3((p.N + 63) / 64, (p.M + 63) / 64), 256, 0, st>>>(p);
+// The warp writes its staged chunk, rows [m, m + 32) and columns [n, n + 64), to a matrix
+// whose rows are not 16-byte aligned: W elements per lane, rows after rows.
+template <int W>
+__device__ __forceinline__ void store_chunk_w(const uint8_t* stg, int lane, void* out, long long stride, long long m,
+                                              int n, int M, int N) {
+  using Raw = typename RawVec<2 * W>::type;
+  constexpr int LANES = 64 / W;  // lanes of a row
+#pragma unroll 4
+  for (int i = lane; i < 32 * LANES; i += 32) {
+    const int r = i / LANES, c = i % LANES * W;
+    if (m + r < M && n + c < N)  // (W divides N: a vector lies inside the row or outside)
+      *reinterpret_cast<Raw*>(static_cast<uint16_t*>(out) + (m + r) * stride + n + c) =
+          *reinterpret_cast<const Raw*>(stg + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+  }
+}
+
+// GEMM on CTA pairs (cluster of 2, tcgen05 cta_group::2): 256 x BN tiles of D, M = 256
+// MMAs spanning both CTAs, each CTA loading its 128 rows of A and half of the B tile by
+// TMA (128-byte swizzle) into an ST-stage ring, fp32 accumulators in TMEM (two of BN
+// columns: the epilogue of a tile runs under the main loop of the next). Eight
+// epilogue warps, two per TMEM lane quarter, take 64-column chunks: 32 values of a
+// row per thread and step, so a block of 32 of a packed pre-activation is one
+// thread's. Waits are bounded; on a timeout the kernel records a status code, waits
+// (bounded) for its own copies and MMAs, frees TMEM and returns.
+template <int BN, bool AMN, bool BMN, typename T>
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_pair_kernel(const __grid_constant__ GemmParams p) {
+  using C = GemmCfg<BN>;
+  constexpr int ST = C::ST;
+  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t IDESC = make_idesc_f16(kBF16, 256, BN, BMN) | (AMN ? 1u << 15 : 0u);
+  constexpr uint32_t SW128 = 2;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+  const int FULL = 0, EMPTY = ST, ACC_FULL = 2 * ST, ACC_EMPTY = 2 * ST + 2, DRAIN = 2 * ST + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(bar(FULL + i), 1);   // the leader's producer arrives; both CTAs' bytes complete it
+      mbar_init(bar(EMPTY + i), 1);  // multicast commit of the leader's MMAs
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(ACC_FULL + i), 1);
+      mbar_init(bar(ACC_EMPTY + i), 2 * kGemmEpiWarps);  // epilogue warps of both CTAs (used in the leader)
+    }
+    mbar_init(bar(DRAIN), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&p.tma_a);
+    tma_prefetch_desc(&p.tma_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // barriers of both CTAs initialised, TMEM allocated
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------------------------------------------------- producer (both CTAs)
+      uint32_t it = 0;
+      bool ok = true;
+      for (Segments s(p, pair, pairs); ok && s.next();) {
+        const int m0 = (s.t / p.tiles_n) * 256 + 128 * static_cast<int>(rank);
+        const int n0 = (s.t % p.tiles_n) * BN + BN / 2 * static_cast<int>(rank);
+        for (int kb = s.k0; kb < s.k1; ++kb, ++it) {
+          const int st = it % ST;
+          if (!gemm_wait(bar(EMPTY + st), ((it / ST) & 1) ^ 1, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x71)) {
+            ok = false;
+            break;
+          }
+          if (leader) mbar_arrive_expect_tx(bar(FULL + st), 2 * C::STAGE);
+          const uint32_t full0 = mapa_shared(bar(FULL + st), 0);  // the leader's stage barrier
+          const uint32_t a = smem_u32(smem + st * C::STAGE), b = a + C::A_BYTES;
+          if constexpr (AMN) {  // two boxes of 64 columns x 64 rows of the reduction
+            tma_load_2d_pair(a, &p.tma_a, full0, m0, kb * C::BK);
+            tma_load_2d_pair(a + 8192, &p.tma_a, full0, m0 + 64, kb * C::BK);
+          } else {
+            tma_load_2d_pair(a, &p.tma_a, full0, kb * C::BK, m0);
+          }
+          if constexpr (BMN) {
+#pragma unroll
+            for (int j = 0; j < BN / 128; ++j)
+              tma_load_2d_pair(b + 8192 * j, &p.tma_b, full0, n0 + 64 * j, kb * C::BK);
+          } else {
+            tma_load_2d_pair(b, &p.tma_b, full0, kb * C::BK, n0);
+          }
+        }
+      }
+      if (leader) {  // copies of both CTAs still in flight land before the pair exits
+        const uint32_t first = it > static_cast<uint32_t>(ST) ? it - ST : 0;
+        for (uint32_t i = first; i < it; ++i) gemm_drain(bar(FULL + i % ST), (i / ST) & 1, p.wait_limit_ns);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // ---------------------------------------------------------- MMA issuer (leader)
+      uint32_t it = 0, lt = 0;
+      bool ok = true;
+      for (Segments s(p, pair, pairs); ok && s.next(); ++lt) {
+        const int buf = lt & 1;
+        if (!gemm_wait(bar(ACC_EMPTY + buf), ((lt >> 1) & 1) ^ 1, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x72))
+          break;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * 256u;
+        for (int kb = s.k0; kb < s.k1; ++kb, ++it) {
+          const int st = it % ST;
+          if (!gemm_wait(bar(FULL + st), (it / ST) & 1, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x73)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = smem_u32(smem + st * C::STAGE);
+          // K-major: 8-row groups 1024 B apart, a K = 16 step is 32 B inside the swizzle atom.
+          // MN-major: 64-column blocks 8192 B apart, 8-row groups of k 1024 B, a step is two of them.
+          const uint64_t ad = make_sdesc(a, AMN ? 8192 : 16, 1024, SW128);
+          const uint64_t bd = make_sdesc(a + C::A_BYTES, BMN ? 8192 : 16, 1024, SW128);
+#pragma unroll
+          for (int kk = 0; kk < C::BK / 16; ++kk)
+            umma_ss_pair(d, ad + (AMN ? 128 : 2) * kk, bd + (BMN ? 128 : 2) * kk, IDESC, (kb - s.k0) | kk);
+          umma_commit_pair_mc(bar(EMPTY + st), 0x3);
+        }
+        if (ok) umma_commit_pair_mc(bar(ACC_FULL + buf), 0x3);
+      }
+      umma_commit_pair_mc(bar(DRAIN), 0x1);
+      gemm_drain(bar(DRAIN), 0, p.wait_limit_ns);
+    }
+  } else {
+    // -------------------------------------------------------------- epilogue (both CTAs)
+    const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;  // TMEM lane quarter, column half
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t acc_empty0 = mapa_shared(bar(ACC_EMPTY), 0);
+    uint8_t* stg = smem + C::OFF_STG + ew * 2 * C::STG;
+    float* bias_s = reinterpret_cast<float*>(smem + C::OFF_BIAS) + ew * 64;
+    const long long nb = pack_blocks(p.N);
+    int sbuf = 0;  // staging buffer of the next chunk
+    uint32_t lt = 0;
+    for (Segments s(p, pair, pairs); s.next(); ++lt) {
+      const int buf = lt & 1;
+      const int m0 = (s.t / p.tiles_n) * 256 + 128 * static_cast<int>(rank) + quarter * 32;
+      const int n0 = (s.t % p.tiles_n) * BN + half * (BN / 2);
+      const long long row = m0 + lane;
+      const bool in_row = row < p.M;
+      const bool ok = gemm_wait(bar(ACC_FULL + buf), (lt >> 1) & 1, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x74);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const uint32_t acc = lane_base + buf * 256u + half * (BN / 2);
+#pragma unroll 1
+      for (int ch = 0; ch < C::CHUNKS; ++ch) {
+        const int n = n0 + 64 * ch;
+        const bool last = ch == C::CHUNKS - 1;
+        if (!s.whole()) {
+          // a part of a tile: fp32 sums into the pair's slot
+          float* dst = p.partial + ((static_cast<size_t>(2 * pair + (s.k0 ? 0 : 1)) * 256 + 128 * rank + quarter * 32 +
+                                     lane) * BN + half * (BN / 2) + 64 * ch);
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[32];
+            tmem_ld32(acc + 64 * ch + 32 * h, v);
+            tmem_ld_wait();
+            if (in_row && n + 32 * h < p.N) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                reinterpret_cast<uint4*>(dst + 32 * h)[c] = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+            }
+          }
+          if (last) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * buf);
+          }
+          continue;
+        }
+        if (n < p.N) {
+          if (p.bias) {
+            __syncwarp();
+            bias_s[lane] = n + lane < p.N ? elem_f32<T>(static_cast<const T*>(p.bias)[n + lane]) : 0.f;
+            bias_s[32 + lane] = n + 32 + lane < p.N ? elem_f32<T>(static_cast<const T*>(p.bias)[n + 32 + lane]) : 0.f;
+          }
+          // the staging buffers this chunk writes: the TMA stores that read them are done
+          if (lane == 0) {
+            if (p.z) bulk_wait_read_all();
+            else bulk_wait_read_but_one();
+          }
+          __syncwarp();
+        }
+        uint8_t* out_s = stg + (p.z ? 1 : sbuf) * C::STG;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          const int c0 = n + 32 * h;
+          uint4 rr[4];
+          if (p.res && p.res_vec && in_row && c0 < p.N) {
+            const T* rp = static_cast<const T*>(p.res) + row * p.res_stride + c0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              rr[c] = c0 + 8 * c < p.N ? *reinterpret_cast<const uint4*>(rp + 8 * c) : make_uint4(0, 0, 0, 0);
+          }
+          uint32_t raw[32];
+          tmem_ld32(acc + 64 * ch + 32 * h, raw);
+          tmem_ld_wait();
+          if (last && h == 1) {  // this warp's last read of the accumulator
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * buf);
+          }
+          if (c0 >= p.N) continue;
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
+          if (p.bias) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 b = reinterpret_cast<const float4*>(bias_s + 32 * h)[i];
+              v[4 * i] += b.x;
+              v[4 * i + 1] += b.y;
+              v[4 * i + 2] += b.z;
+              v[4 * i + 3] += b.w;
+            }
+          }
+          if (p.z) stage32<T>(stg, lane, h, v);
+          if (p.z_codes) {
+            // (columns past N hold zeros: W's rows there are read as zeros, the bias too)
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) m = max(m, abs_bits(v[i]));
+            const uint32_t sc = pack_scale(m);
+            const float inv = pack_inv(sc), lim = pack_limit(sc);
+            if (in_row) {
+              uint4* dst = reinterpret_cast<uint4*>(p.z_codes + (row * nb + c0 / 32) * kPackBlock);
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                uint4 w;
+                w.x = pack_code4(v[16 * c], v[16 * c + 1], v[16 * c + 2], v[16 * c + 3], inv, lim);
+                w.y = pack_code4(v[16 * c + 4], v[16 * c + 5], v[16 * c + 6], v[16 * c + 7], inv, lim);
+                w.z = pack_code4(v[16 * c + 8], v[16 * c + 9], v[16 * c + 10], v[16 * c + 11], inv, lim);
+                w.w = pack_code4(v[16 * c + 12], v[16 * c + 13], v[16 * c + 14], v[16 * c + 15], inv, lim);
+                dst[c] = w;
+              }
+              p.z_scales[row * nb + c0 / 32] = static_cast<uint8_t>(sc);
+            }
+          }
+          act_any(p.act, v);
+          if (p.res && in_row) {
+            if (p.res_vec) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                float f[8];
+                unpack8<T>(rr[c], f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[8 * c + e] += f[e];
+              }
+            } else {
+              const T* rp = static_cast<const T*>(p.res) + row * p.res_stride + c0;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c0 + i < p.N) v[i] += elem_f32<T>(rp[i]);
+            }
+          }
+          stage32<T>(out_s, lane, h, v);
+        }
+        if (n >= p.N) continue;
+        fence_proxy_async_smem();  // staging writes visible to the TMA stores
+        __syncwarp();
+        if (lane == 0 && m0 < p.M) {
+          if (p.z && p.z_tma) tma_store_2d(&p.tma_z, smem_u32(stg), n, m0);
+          if (p.out_tma) tma_store_2d(&p.tma_out, smem_u32(out_s), n, m0);
+        }
+        if (lane == 0) bulk_commit_group();
+        if (p.z && !p.z_tma) {
+          if (p.z_w == 4) store_chunk_w<4>(stg, lane, p.z, p.z_stride, m0, n, p.M, p.N);
+          else if (p.z_w == 2) store_chunk_w<2>(stg, lane, p.z, p.z_stride, m0, n, p.M, p.N);
+          else store_chunk_w<1>(stg, lane, p.z, p.z_stride, m0, n, p.M, p.N);
+        }
+        if (!p.out_tma) {
+          if (p.out_w == 4) store_chunk_w<4>(out_s, lane, p.out, p.out_stride, m0, n, p.M, p.N);
+          else if (p.out_w == 2) store_chunk_w<2>(out_s, lane, p.out, p.out_stride, m0, n, p.M, p.N);
+          else store_chunk_w<1>(out_s, lane, p.out, p.out_stride, m0, n, p.M, p.N);
+        }
+        sbuf ^= 1;
+      }
+    }
+    if (lane == 0) bulk_wait_all();  // output written before the CTA ends
+  }
+  tc_fence_before();
+  cluster_sync_all();  // no CTA leaves while its pair may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// Joins the parts of split tiles in the order of k and applies the epilogue: eight
+// columns of a row per thread, four neighbouring threads a block of 32 columns.
+template <int BN, typename T>
+__global__ void __launch_bounds__(256) gemm_finish_kernel(const __grid_constant__ GemmParams p) {
+  const int t = blockIdx.x;
+  const int first = static_cast<int>(static_cast<long long>(t) * p.nk / p.split);
+  const int last = static_cast<int>((static_cast<long long>(t + 1) * p.nk - 1) / p.split);
+  if (first == last) return;  // one pair computed the whole tile
+  const int m0 = (t / p.tiles_n) * 256, n0 = (t % p.tiles_n) * BN;
+  const long long nb = pack_blocks(p.N);
+  constexpr int PER_ROW = BN / 8;
+  constexpr int ROWS = 256 / PER_ROW;  // rows of one pass of the block
+  const int c = static_cast<int>(threadIdx.x) % PER_ROW * 8, n = n0 + c;
+  for (int r = blockIdx.y * ROWS + static_cast<int>(threadIdx.x) / PER_ROW; r < 256; r += gridDim.y * ROWS) {
+    const long long row = m0 + r;
+    if (m0 + r - static_cast<int>(threadIdx.x) / PER_ROW >= p.M) break;  // (the same for the whole block)
+    const bool in = row < p.M && n < p.N;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (in) {
+      for (int q = first; q <= last; ++q) {
+        const long long b = static_cast<long long>(q) * p.split;
+        const int slot = 2 * q + (b > static_cast<long long>(t) * p.nk ? 0 : 1);  // began inside the tile, or before or at its first step
+        const float4* src = reinterpret_cast<const float4*>(p.partial + (static_cast<size_t>(slot) * 256 + r) * BN + c);
+        const float4 x = __ldcg(src), y = __ldcg(src + 1);
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (in && n + i < p.N) {
+        if (p.bias) v[i] += elem_f32<T>(static_cast<const T*>(p.bias)[n + i]);
+      } else {
+        v[i] = 0.f;
+      }
+    }
+    if (p.z_codes) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const uint32_t sc = pack_scale(m);
+      const float inv = pack_inv(sc), lim = pack_limit(sc);
+      if (row < p.M && n < nb * kPackBlock) {
+        uint2 w;
+        w.x = pack_code4(v[0], v[1], v[2], v[3], inv, lim);
+        w.y = pack_code4(v[4], v[5], v[6], v[7], inv, lim);
+        *reinterpret_cast<uint2*>(p.z_codes + row * nb * kPackBlock + n) = w;
+        if (n % kPackBlock == 0) p.z_scales[row * nb + n / kPackBlock] = static_cast<uint8_t>(sc);
+      }
+    }
+    if (!in) continue;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = v[i];
+    act_any(p.act, y);
+    if (p.res) {
+      const T* rp = static_cast<const T*>(p.res) + row * p.res_stride + n;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < p.N) y[i] += elem_f32<T>(rp[i]);
+    }
+    auto put = [&](void* base, long long stride, const float (&f)[8], int wide) {
+      T* dst = static_cast<T*>(base) + row * stride + n;
+      if (wide) {
+        uint4 w;
+        w.x = pack2<T>(f[0], f[1]);
+        w.y = pack2<T>(f[2], f[3]);
+        w.z = pack2<T>(f[4], f[5]);
+        w.w = pack2<T>(f[6], f[7]);
+        *reinterpret_cast<uint4*>(dst) = w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (n + i < p.N) dst[i] = f32_elem<T>(f[i]);
+      }
+    };
+    if (p.z) put(p.z, p.z_stride, v, p.z_tma && n + 8 <= p.N);
+    put(p.out, p.out_stride, y, p.out_tma && n + 8 <= p.N);
+  }
+}
+
+// ---------------------------------------------------------------- host
+// One operand or output of a product: rows of `stride` elements.
+struct Mat {
+  const void* p;
+  long long stride;
+};
+
+int encode_map(CUtensorMap* m, const void* base, long long cols, long long rows, long long stride, int box_cols,
+               int box_rows, bool bf16) {
+  const TmapEncodeFn enc = tmap_encoder();
+  if (!enc) return FRATTN_E_TMAP;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : FRATTN_E_TMAP;
+}
+
+bool rows16(const void* p, long long stride) { return aligned_to(p, 16) && stride % 8 == 0; }
+
+int sm_pairs() {
+  const int n = sm_count_for_current_device();
+  return (n > 1 ? n : 148) / 2;
+}
+
+// Tile width and split of an M x N product over nk steps of 64.
+struct GemmPlan {
+  int bn, tiles, split, pairs;
+  size_t partial_bytes;
+};
+
+GemmPlan gemm_plan(int M, int N, int nk) {
+  GemmPlan best{};
+  const int P = sm_pairs();
+  double best_us = 1e30;
+  for (int bn : {256, 128}) {
+    const long long tiles = static_cast<long long>((M + 255) / 256) * ((N + bn - 1) / bn);
+    if (tiles > (1 << 30) / (nk + 1)) continue;
+    const double step_us = bn == 256 ? 0.36 : 0.21;  // one 64-wide step of a 256 x bn tile
+    {
+      const long long waves = (tiles + P - 1) / P;
+      const double us = static_cast<double>(waves) * nk * step_us + 2.0;
+      if (us < best_us) {
+        best_us = us;
+        best = GemmPlan{bn, static_cast<int>(tiles), 0, static_cast<int>(tiles < P ? tiles : P), 0};
+      }
+    }
+    const long long total = tiles * nk;
+    int split = static_cast<int>((total + P - 1) / P);
+    if (split < 4) split = 4;
+    if (split < nk && tiles % P != 0) {
+      const int pairs = static_cast<int>((total + split - 1) / split);
+      const double rows = M < 256 ? M : 256;
+      const double us = split * step_us + 6.0 + 2.0 * pairs * rows * bn * 4 * 2 / 4e6;
+      if (us < best_us) {
+        best_us = us;
+        best = GemmPlan{bn, static_cast<int>(tiles), split, pairs, static_cast<size_t>(2) * pairs * 256 * bn * 4};
+      }
+    }
+  }
+  return best;
+}
+
+template <int BN, bool AMN, bool BMN, typename T>
+int gemm_launch(GemmParams& p, const GemmPlan& plan, cudaStream_t st) {
+  using C = GemmCfg<BN>;
+  auto kern = gemm_pair_kernel<BN, AMN, BMN, T>;
+  static unsigned long long attr_set = 0;  // per device; setting twice is harmless
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bitv = 1ull << (dev & 63);
+  if (!(attr_set & bitv)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+      return FRATTN_E_CUDA;
+    attr_set |= bitv;
+  }
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(2 * plan.pairs);
+  lc.blockDim = dim3(kGemmThreads);
+  lc.dynamicSmemBytes = C::SMEM;
+  lc.stream = st;
+  lc.attrs = &attr;
+  lc.numAttrs = 1;
+  if (cudaLaunchKernelEx(&lc, kern, p) != cudaSuccess) return FRATTN_E_CUDA;
+  if (plan.split) gemm_finish_kernel<BN, T><<<dim3(plan.tiles, 8), 256, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : FRATTN_E_CUDA;
 }
+
+// D[M, N] = A B^T with the epilogue in p (bias .. z_scales set by the caller). A is
+// [M, K] rows (or [K, M] with AMN), B [N, K] (or [K, N] with BMN), 16-byte rows.
+template <bool AMN, bool BMN, typename T>
+int gemm(GemmParams& p, const Mat& a, const Mat& b, int M, int N, int K, void* ws, size_t ws_bytes, int32_t* status,
+         cudaStream_t st) {
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  p.M = M;
+  p.N = N;
+  p.nk = (K + 63) / 64;
+  const GemmPlan plan = gemm_plan(M, N, p.nk);
+  if (!plan.bn) return FRATTN_E_SHAPE;
+  if (plan.partial_bytes > ws_bytes) return FRATTN_E_WORKSPACE;
+  p.tiles_n = (N + plan.bn - 1) / plan.bn;
+  p.tiles = plan.tiles;
+  p.split = plan.split;
+  p.partial = static_cast<float*>(ws);
+  p.status = status;
+  p.wait_limit_ns = frattn_wait_limit_ns();
+  if (encode_map(&p.tma_a, a.p, AMN ? M : K, AMN ? K : M, a.stride, 64, AMN ? 64 : 128, bf16) ||
+      encode_map(&p.tma_b, b.p, BMN ? N : K, BMN ? K : N, b.stride, 64, BMN ? 64 : plan.bn / 2, bf16))
+    return FRATTN_E_TMAP;
+  auto width = [&](const void* q, long long stride) {
+    for (int w = 4; w > 1; w >>= 1)
+      if (aligned_to(q, 2 * w) && stride % w == 0 && N % w == 0) return w;
+    return 1;
+  };
+  p.out_tma = rows16(p.out, p.out_stride);
+  p.out_w = width(p.out, p.out_stride);
+  if (p.out_tma && encode_map(&p.tma_out, p.out, N, M, p.out_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
+  if (p.z) {
+    p.z_tma = rows16(p.z, p.z_stride);
+    p.z_w = width(p.z, p.z_stride);
+    if (p.z_tma && encode_map(&p.tma_z, p.z, N, M, p.z_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
+  }
+  // (a vector of 8 may then start inside the row and end past it: only where N % 8 == 0)
+  p.res_vec = p.res && rows16(p.res, p.res_stride) && N % 8 == 0;
+  if (plan.bn == 256) return gemm_launch<256, AMN, BMN, T>(p, plan, st);
+  return gemm_launch<128, AMN, BMN, T>(p, plan, st);
+}
+
+size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 // dz = dout act'(z) over rows of N columns, with partial column sums of dz.
 struct ActBwdParams {
@@ -230,13 +805,12 @@ int act_bwd(const ActBwdParams& p, int act, int* groups, cudaStream_t st) {
   return p.z_codes ? act_bwd_act<T, 1, true>(p, act, groups, st) : act_bwd_act<T, 1, false>(p, act, groups, st);
 }
 
-size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
-
 // Workspace of the backward pass: dz [T, Np] (rows padded to 16 bytes), partial
-// column sums, and the 16-bit values of a packed x [T, Kp].
+// column sums, the 16-bit values of a packed x [T, Kp], and the parts of split tiles
+// (of one product at a time).
 struct BwdLayout {
   long long np, kp;
-  size_t dz, partial, x, total;
+  size_t dz, partial, x, gemm, gemm_bytes, total;
 };
 BwdLayout bwd_layout(int T, int K, int N) {
   BwdLayout l;
@@ -245,7 +819,11 @@ BwdLayout bwd_layout(int T, int K, int N) {
   l.dz = 0;
   l.partial = up256(static_cast<size_t>(T) * l.np * 2);
   l.x = l.partial + up256(static_cast<size_t>(kMaxStrips) * N * sizeof(float));
-  l.total = l.x + up256(static_cast<size_t>(T) * l.kp * 2);
+  l.gemm = l.x + up256(static_cast<size_t>(T) * l.kp * 2);
+  const size_t dx = gemm_plan(T > 0 ? T : 1, K, (N + 63) / 64).partial_bytes;
+  const size_t dw = gemm_plan(N, K, T > 0 ? (T + 63) / 64 : 1).partial_bytes;
+  l.gemm_bytes = dx > dw ? dx : dw;
+  l.total = l.gemm + up256(l.gemm_bytes);
   return l;
 }
 
@@ -253,9 +831,9 @@ template <typename T>
 int linear_bwd(const void* dout, long long dout_stride, const void* x, long long x_stride, const int8_t* x_codes,
                const uint8_t* x_scales, const void* w, long long w_stride, const void* z, long long z_stride,
                const int8_t* z_codes, const uint8_t* z_scales, int act, int rows, int K, int N, int dtype, void* dx,
-               long long dx_stride, void* dw, void* db, uint8_t* ws, cudaStream_t st) {
+               long long dx_stride, void* dw, void* db, uint8_t* ws, int32_t* status, cudaStream_t st) {
   const BwdLayout l = bwd_layout(rows, K, N);
-  const bool in_place = act == FRATTN_ACT_NONE && aligned_to(dout, 16) && dout_stride % 8 == 0;
+  const bool in_place = act == FRATTN_ACT_NONE && rows16(dout, dout_stride) && dout_stride >= N;
   const void* dz = in_place ? dout : ws + l.dz;
   const long long dz_stride = in_place ? dout_stride : l.np;
   int rc = 0;
@@ -280,46 +858,29 @@ int linear_bwd(const void* dout, long long dout_stride, const void* x, long long
     if (db && (rc = column_finish(reinterpret_cast<float*>(ws + l.partial), groups, 1, N, db, nullptr, dtype, st)))
       return rc;
   }
-  MatmulParams m;
+  GemmParams m;
   if (dx && rows > 0) {
     memset(&m, 0, sizeof(m));
-    m.a = dz;
-    m.a_m = dz_stride;
-    m.a_k = 1;
-    m.b = w;
-    m.b_n = 1;
-    m.b_k = w_stride;
-    m.M = rows;
-    m.N = K;
-    m.K = N;
     m.out = dx;
     m.out_stride = dx_stride;
-    if ((rc = matmul<T>(m, st))) return rc;
+    const Mat a{dz, dz_stride}, b{w, w_stride};
+    if ((rc = gemm<false, true, T>(m, a, b, rows, K, N, ws + l.gemm, l.gemm_bytes, status, st))) return rc;
   }
   if (dw) {
-    if (x_codes && rows > 0) {
+    if (rows == 0) return cudaMemsetAsync(dw, 0, static_cast<size_t>(N) * K * 2, st) == cudaSuccess ? 0 : FRATTN_E_CUDA;
+    if (x_codes) {
       if ((rc = act_unpack(x_codes, x_scales, rows, K, dtype, ws + l.x, l.kp, st))) return rc;
       x = ws + l.x;
       x_stride = l.kp;
     }
     memset(&m, 0, sizeof(m));
-    m.a = dz;
-    m.a_m = 1;
-    m.a_k = dz_stride;
-    m.b = x;
-    m.b_n = 1;
-    m.b_k = x_stride;
-    m.M = N;
-    m.N = K;
-    m.K = rows;
     m.out = dw;
     m.out_stride = K;
-    if ((rc = matmul<T>(m, st))) return rc;
+    const Mat a{dz, dz_stride}, b{x, x_stride};
+    return gemm<true, true, T>(m, a, b, N, K, rows, ws + l.gemm, l.gemm_bytes, status, st);
   }
   return 0;
 }
-
-bool rows16(const void* p, long long stride) { return aligned_to(p, 16) && stride % 8 == 0; }
 
 }  // namespace
 }  // namespace frattn
@@ -331,7 +892,7 @@ extern "C" {
 int frattn_workspace_bytes_linear_act(int T, int K, int N, size_t* bytes) {
   if (!bytes) return FRATTN_E_NULL;
   if (T < 0 || K <= 0 || N <= 0) return FRATTN_E_SHAPE;
-  *bytes = 0;
+  *bytes = T > 0 ? gemm_plan(T, N, (K + 63) / 64).partial_bytes : 0;
   return 0;
 }
 
@@ -351,19 +912,10 @@ int frattn_linear_act(const void* x, long long x_stride, const void* w, long lon
   size_t need = 0;
   frattn_workspace_bytes_linear_act(T, K, N, &need);
   if (workspace_bytes < need) return FRATTN_E_WORKSPACE;
-  (void)workspace;
-  (void)status;
-  MatmulParams m;
+  if (need && !workspace) return FRATTN_E_NULL;
+  if (!aligned_to(workspace, 256)) return FRATTN_E_ALIGN;
+  GemmParams m;
   memset(&m, 0, sizeof(m));
-  m.a = x;
-  m.a_m = x_stride;
-  m.a_k = 1;
-  m.b = w;
-  m.b_n = w_stride;
-  m.b_k = 1;
-  m.M = T;
-  m.N = N;
-  m.K = K;
   m.bias = bias;
   m.res = residual;
   m.res_stride = res_stride;
@@ -375,7 +927,10 @@ int frattn_linear_act(const void* x, long long x_stride, const void* w, long lon
   m.z_codes = z_codes;
   m.z_scales = z_scales;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == FRATTN_BF16 ? matmul<__nv_bfloat16>(m, st) : matmul<__half>(m, st);
+  const Mat a{x, x_stride}, b{w, w_stride};
+  if (dtype == FRATTN_BF16)
+    return gemm<false, false, __nv_bfloat16>(m, a, b, T, N, K, workspace, workspace_bytes, status, st);
+  return gemm<false, false, __half>(m, a, b, T, N, K, workspace, workspace_bytes, status, st);
 }
 
 int frattn_workspace_bytes_linear_act_bwd(int T, int K, int N, size_t* bytes) {
@@ -407,14 +962,13 @@ int frattn_linear_act_bwd(const void* dout, long long dout_stride, const void* x
   size_t need = 0;
   frattn_workspace_bytes_linear_act_bwd(T, K, N, &need);
   if (workspace_bytes < need) return FRATTN_E_WORKSPACE;
-  (void)status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (dtype == FRATTN_BF16)
     return linear_bwd<__nv_bfloat16>(dout, dout_stride, x, x_stride, x_codes, x_scales, w, w_stride, z, z_stride,
-                                     z_codes, z_scales, activation, T, K, N, dtype, dx, dx_stride, dw, db, ws, st);
+                                     z_codes, z_scales, activation, T, K, N, dtype, dx, dx_stride, dw, db, ws, status, st);
   return linear_bwd<__half>(dout, dout_stride, x, x_stride, x_codes, x_scales, w, w_stride, z, z_stride, z_codes,
-                            z_scales, activation, T, K, N, dtype, dx, dx_stride, dw, db, ws, st);
+                            z_scales, activation, T, K, N, dtype, dx, dx_stride, dw, db, ws, status, st);
 }
 
 }  // extern "C"

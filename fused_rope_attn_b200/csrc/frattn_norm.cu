@@ -418,13 +418,13 @@ __global__ void __launch_bounds__(256) act_pack_kernel(const PackParams p) {
 #pragma unroll
       for (int o = G / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
       const uint32_t scale = pack_scale(m);
-      const float inv = pack_inv(scale);
+      const float inv = pack_inv(scale), lim = pack_limit(scale);
       union {
         typename RawVec<VEC == 1 ? 2 : VEC>::type raw;
         int8_t c[VEC == 1 ? 2 : VEC];
       } o;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o.c[e] = has && row < p.T ? static_cast<int8_t>(pack_code(x[r].get(e), inv)) : 0;
+      for (int e = 0; e < VEC; ++e) o.c[e] = has && row < p.T ? static_cast<int8_t>(pack_code(x[r].get(e), inv, lim)) : 0;
       if (in_row && row < p.T) {
         int8_t* dst = p.codes + row * nb * kPackBlock + static_cast<size_t>(v) * VEC;
         if constexpr (VEC == 1) *dst = o.c[0];

@@ -481,3 +481,22 @@ def test_gpu_refusals():
             print("accepted:", i)
     torch.cuda.synchronize()
     assert last_status(DEV) == 0
+
+
+def test_gradients_of_broadcast_outputs():
+    """y.sum().backward() hands an expanded gradient (strides 0) to the nodes, and a
+    gradient whose rows are one row repeated (row stride 0) is read in place."""
+    x, w, b, _ = linear_inputs(70, 64, 48, BF, True, False)
+    ps = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    fr.linear_act_train(*ps, activation="relu").sum().backward()
+    one = torch.ones(70, 48, dtype=BF, device=DEV)
+    z = fr.linear_act(*gpu(x, w, b), save_preact="full")[1]
+    ref = fr.linear_act_backward(one, x.to(DEV), w.to(DEV), z, activation="relu")
+    assert all(torch.equal(p.grad, r) for p, r in zip(ps, ref))
+    for act in ("none", "relu"):
+        got = fr.linear_act_backward(one[:1].expand(70, 48), x.to(DEV), w.to(DEV), z, activation=act)
+        ref = fr.linear_act_backward(one, x.to(DEV), w.to(DEV), z, activation=act)
+        assert all(torch.equal(s, t) for s, t in zip(got, ref))
+    nx = x.to(DEV).requires_grad_(True)
+    fr.layer_norm_train(nx).sum().backward()
+    assert nx.grad.abs().max() <= 2.0 ** -6  # the sum of a row's outputs is constant
