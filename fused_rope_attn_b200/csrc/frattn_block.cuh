@@ -132,7 +132,47 @@ __device__ __forceinline__ uint32_t pack_code4(float a, float b, float c, float 
   return __byte_perm(lo, hi, 0x5410);
 }
 
+// max(m, |a|, |b|); a NaN among them stays.
+__device__ __forceinline__ float max3_abs(float m, float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+// A whole block of 32 held by one thread: its codes (four to a word) and scale byte.
+// Two values at a time on the packed fp32 pipe; the limit to 127 steps, which only a
+// block whose largest magnitude is within 2^-7 of a power of two needs, is a branch.
+__device__ __forceinline__ uint32_t pack32(const float (&v)[32], uint32_t (&codes)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) m = max3_abs(m, v[i], v[i + 1]);
+  const uint32_t sc = pack_scale(abs_bits(m));
+  const float inv = pack_inv(sc);
+  if (fabsf(m) * inv < 127.5f) {  // (false for a NaN block: infinity x 0)
+    const uint64_t inv2 = f2pack(inv, inv), magic = f2pack(12582912.f, 12582912.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float a, b, c, d;
+      f2unpack(fma2(f2pack(v[4 * i], v[4 * i + 1]), inv2, magic), a, b);
+      f2unpack(fma2(f2pack(v[4 * i + 2], v[4 * i + 3]), inv2, magic), c, d);
+      const uint32_t lo = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
+      const uint32_t hi = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+      codes[i] = __byte_perm(lo, hi, 0x5410);
+    }
+  } else {
+    const float lim = pack_limit(sc);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) codes[i] = pack_code4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv, lim);
+  }
+  return sc;
+}
+
 // ---------------------------------------------------------------- activations
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t both(float x) { return f2pack(x, x); }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -177,6 +217,44 @@ __device__ __forceinline__ float act_f(float z) {
     return z * sigmoid_f(z);
   } else {
     return z;
+  }
+}
+
+// Two values at a time: the polynomial parts on the packed fp32 pipe.
+template <int ACT>
+__device__ __forceinline__ void act_f2(float& a, float& b) {
+  if constexpr (ACT == FRATTN_ACT_GELU) {  // normal_cdf's steps
+    const uint64_t z = f2pack(a, b);
+    float t0, t1, e0, e1, q0, q1;
+    f2unpack(fma2(f2pack(fabsf(a), fabsf(b)), both(0.23164191f), both(1.f)), t0, t1);
+    const uint64_t t = f2pack(rcp_fast(t0), rcp_fast(t1));
+    f2unpack(mul2(mul2(z, both(-0.7213475204444817f)), z), e0, e1);
+    const uint64_t e = f2pack(exp2_fast(e0), exp2_fast(e1));
+    uint64_t q = fma2(t, both(0.5307027145f), both(-0.7265760135f));
+    q = fma2(q, t, both(0.7107068705f));
+    q = fma2(q, t, both(-0.142248368f));
+    q = fma2(q, t, both(0.127414796f));
+    f2unpack(mul2(mul2(q, t), e), q0, q1);
+    a *= a < 0.f ? q0 : 1.f - q0;
+    b *= b < 0.f ? q1 : 1.f - q1;
+  } else if constexpr (ACT == FRATTN_ACT_GELU_TANH) {
+    const uint64_t z = f2pack(a, b);
+    uint64_t u = fma2(mul2(z, z), both(-0.10294324f), both(-2.3022082f));  // -2 sqrt(2 / pi) log2(e) (0.044715 z^2 + 1)
+    u = mul2(u, z);
+    float u0, u1;
+    f2unpack(u, u0, u1);
+    f2unpack(add2(f2pack(exp2_fast(u0), exp2_fast(u1)), both(1.f)), u0, u1);
+    a *= rcp_fast(u0);
+    b *= rcp_fast(u1);
+  } else if constexpr (ACT == FRATTN_ACT_SILU) {
+    float u0, u1;
+    f2unpack(mul2(f2pack(a, b), both(-1.4426950408889634f)), u0, u1);
+    f2unpack(add2(f2pack(exp2_fast(u0), exp2_fast(u1)), both(1.f)), u0, u1);
+    a *= rcp_fast(u0);
+    b *= rcp_fast(u1);
+  } else {
+    a = act_f<ACT>(a);
+    b = act_f<ACT>(b);
   }
 }
 

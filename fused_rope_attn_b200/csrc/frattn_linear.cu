@@ -18,7 +18,8 @@ int act_unpack(const int8_t* codes, const uint8_t* scales, int T, int C, int dty
 // forward product), "MN-major" when they run along m or n (W in dz W, both in dz^T x).
 struct GemmParams {
   CUtensorMap tma_a, tma_b;
-  CUtensorMap tma_out, tma_z;  // box {64, 32}, 128-byte swizzle; used where out_tma / z_tma
+  CUtensorMap tma_out, tma_z, tma_res;  // box {64, 32}, 128-byte swizzle; used where *_tma
+  CUtensorMap tma_codes;                // box {64, 32} bytes, 64-byte swizzle
   const void* bias;            // [N] or null
   const void* res;             // [M, N] or null
   long long res_stride;
@@ -29,9 +30,9 @@ struct GemmParams {
   long long z_stride;
   int8_t* z_codes;  // or null
   uint8_t* z_scales;
-  int out_tma, z_tma;          // written by TMA stores (16-byte rows), else element stores of
+  int out_tma, z_tma;          // written by TMA stores (16-byte rows), else by element stores of
   int out_w, z_w;              // 4, 2 or 1 elements
-  int res_vec;                 // residual rows are 16-byte aligned
+  int res_tma;                 // residual read ahead by TMA (16-byte rows, nothing else staged)
   int M, N, nk;                // nk: 64-wide steps of the reduction
   int tiles_n, tiles;
   int split;                   // 0: a pair owns whole tiles; else k steps per pair (see Segments)
@@ -42,27 +43,25 @@ struct GemmParams {
 
 namespace {
 
-constexpr int kGemmThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
-constexpr int kGemmEpiWarps = 8;
-
 template <int BN>
 struct GemmCfg {
   static constexpr int BK = 64;
   static constexpr int A_BYTES = 128 * BK * 2;
   static constexpr int B_BYTES = BN / 2 * BK * 2;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int CHUNKS = BN / 128;           // 64-column chunks per epilogue warp and tile
-  static constexpr int STG = 32 * 64 * 2;           // one warp's 32 x 64 output chunk
-  static constexpr int STG_BYTES = kGemmEpiWarps * 2 * STG;
-  static constexpr int BIAS_BYTES = kGemmEpiWarps * 64 * 4;
+  static constexpr int EPI_WARPS = 4 * ((BN + 63) / 64);  // four lane quarters x 64-column chunks
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;      // warp 0 TMA, warp 1 MMA, the rest epilogue
+  static constexpr int STG = 32 * 64 * 2;                  // a warp's staging: 32 rows x 64 columns of 16 bits
+  static constexpr int STG_BYTES = EPI_WARPS * STG;
+  static constexpr int BIAS_BYTES = EPI_WARPS * 64 * 4;
   static constexpr int ST_FIT = (227 * 1024 - 1024 - 512 - STG_BYTES - BIAS_BYTES) / STAGE;
   static constexpr int ST = ST_FIT > 8 ? 8 : ST_FIT;
   static constexpr int OFF_STG = ST * STAGE;
   static constexpr int OFF_BIAS = OFF_STG + STG_BYTES;
   static constexpr int OFF_BAR = OFF_BIAS + BIAS_BYTES;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;  // barriers + 1024-B alignment slack
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;  // barriers + 1024-B alignment slack
   static_assert(STAGE % 1024 == 0 && OFF_STG % 1024 == 0, "128-B swizzle atoms");
-  static_assert((2 * ST + 5) * 8 + 8 <= 256, "barriers");
+  static_assert((2 * ST + 5 + EPI_WARPS) * 8 + 8 <= 512, "barriers");
 };
 
 // The tiles (or parts of tiles) a CTA pair computes, in order; every role of the
@@ -139,7 +138,7 @@ __device__ __forceinline__ void gemm_drain(uint32_t bar, uint32_t parity, unsign
 template <int ACT, int N>
 __device__ __forceinline__ void act_all(float (&v)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = act_f<ACT>(v[i]);
+  for (int i = 0; i < N; i += 2) act_f2<ACT>(v[i], v[i + 1]);
 }
 template <int N>
 __device__ __forceinline__ void act_any(int act, float (&v)[N]) {
@@ -152,11 +151,15 @@ __device__ __forceinline__ void act_any(int act, float (&v)[N]) {
   }
 }
 
-// 32 values of row r into columns [32 half, 32 half + 32) of a warp's [32][64] 16-bit
-// staging chunk (rows of 128 bytes, 128-byte swizzle: 16-byte piece c of row r lies at
-// c ^ (r & 7), which is what the TMA store expects and spreads the lanes over the banks).
+// A warp's staging holds 32 rows of 64 columns (16 bits: 128 bytes a row, 128-byte
+// swizzle) as the TMA transfers expect it: 16-byte part c of row r lies at c ^ (r & 7),
+// which also spreads the lanes over the banks.
+__device__ __forceinline__ uint4* stage_part(uint8_t* stg, int r, int c) {
+  return reinterpret_cast<uint4*>(stg + r * 128 + ((c ^ (r & 7)) << 4));
+}
+// 32 values of row r into the staging's columns [32 h, 32 h + 32).
 template <typename T>
-__device__ __forceinline__ void stage32(uint8_t* stg, int r, int half, const float (&v)[32]) {
+__device__ __forceinline__ void stage32(uint8_t* stg, int r, int h, const float (&v)[32]) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     uint4 w;
@@ -164,15 +167,15 @@ __device__ __forceinline__ void stage32(uint8_t* stg, int r, int half, const flo
     w.y = pack2<T>(v[8 * c + 2], v[8 * c + 3]);
     w.z = pack2<T>(v[8 * c + 4], v[8 * c + 5]);
     w.w = pack2<T>(v[8 * c + 6], v[8 * c + 7]);
-    *reinterpret_cast<uint4*>(stg + r * 128 + (((4 * half + c) ^ (r & 7)) << 4)) = w;
+    *stage_part(stg, r, 4 * h + c) = w;
   }
 }
 
-// The warp writes its staged chunk, rows [m, m + 32) and columns [n, n + 64), to a matrix
-// whose rows are not 16-byte aligned: W elements per lane, rows after rows.
+// The warp writes its staging, rows [m, m + 32) and columns [n, n + 64), to a matrix
+// whose rows are not 16-byte aligned: W elements per lane, a row's in neighbouring lanes.
 template <int W>
-__device__ __forceinline__ void store_chunk_w(const uint8_t* stg, int lane, void* out, long long stride, long long m,
-                                              int n, int M, int N) {
+__device__ __forceinline__ void store_rows_w(const uint8_t* stg, int lane, void* out, long long stride, long long m,
+                                             int n, int M, int N) {
   using Raw = typename RawVec<2 * W>::type;
   constexpr int LANES = 64 / W;  // lanes of a row
 #pragma unroll 4
@@ -183,17 +186,52 @@ __device__ __forceinline__ void store_chunk_w(const uint8_t* stg, int lane, void
           *reinterpret_cast<const Raw*>(stg + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
   }
 }
+// The staged 16-bit values to a matrix, by TMA where its rows allow.
+__device__ __forceinline__ void store_staged(const CUtensorMap* map, int tma, int width, uint8_t* stg, int lane, void* out,
+                                             long long stride, int m0, int n0, int M, int N) {
+  if (tma) {
+    fence_proxy_async_smem();  // the warp's staging writes, visible to the TMA store
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(map, smem_u32(stg), n0, m0);
+      bulk_commit_group();
+    }
+  } else {
+    __syncwarp();
+    if (width == 4) store_rows_w<4>(stg, lane, out, stride, m0, n0, M, N);
+    else if (width == 2) store_rows_w<2>(stg, lane, out, stride, m0, n0, M, N);
+    else store_rows_w<1>(stg, lane, out, stride, m0, n0, M, N);
+    __syncwarp();
+  }
+}
+// Lane 0's TMA stores have read the staging: the warp may write it again.
+__device__ __forceinline__ void staging_free(int lane) {
+  if (lane == 0) bulk_wait_read_all();
+  __syncwarp();
+}
+
+__device__ __forceinline__ void add_bias(float (&v)[32], const float* bias) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float4 b = reinterpret_cast<const float4*>(bias)[i];
+    v[4 * i] += b.x;
+    v[4 * i + 1] += b.y;
+    v[4 * i + 2] += b.z;
+    v[4 * i + 3] += b.w;
+  }
+}
 
 // GEMM on CTA pairs (cluster of 2, tcgen05 cta_group::2): 256 x BN tiles of D, M = 256
 // MMAs spanning both CTAs, each CTA loading its 128 rows of A and half of the B tile by
 // TMA (128-byte swizzle) into an ST-stage ring, fp32 accumulators in TMEM (two of BN
-// columns: the epilogue of a tile runs under the main loop of the next). Eight
-// epilogue warps, two per TMEM lane quarter, take 64-column chunks: 32 values of a
-// row per thread and step, so a block of 32 of a packed pre-activation is one
-// thread's. Waits are bounded; on a timeout the kernel records a status code, waits
+// columns: the epilogue of a tile runs under the main loop of the next). The epilogue
+// warps each take 64 columns of a TMEM lane quarter, 32 values of a row per thread and
+// step, so a block of 32 of a packed pre-activation is one thread's. (Sixteen warps: with
+// eight of them the epilogue, not the main loop, set the pace of K = 1280 with gelu:
+// two warps to a scheduler leave most of its issue slots empty.) Waits are bounded; on a timeout the kernel records a status code, waits
 // (bounded) for its own copies and MMAs, frees TMEM and returns.
 template <int BN, bool AMN, bool BMN, typename T>
-__global__ void __launch_bounds__(kGemmThreads, 1) gemm_pair_kernel(const __grid_constant__ GemmParams p) {
+__global__ void __launch_bounds__(GemmCfg<BN>::THREADS, 1) gemm_pair_kernel(const __grid_constant__ GemmParams p) {
   using C = GemmCfg<BN>;
   constexpr int ST = C::ST;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
@@ -205,7 +243,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_pair_kernel(const __grid
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   auto bar = [&](int i) { return smem_u32(bars + i); };
   const int FULL = 0, EMPTY = ST, ACC_FULL = 2 * ST, ACC_EMPTY = 2 * ST + 2, DRAIN = 2 * ST + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 5);
+  const int RES = 2 * ST + 5;  // residual chunk of each epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 5 + C::EPI_WARPS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -219,9 +258,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_pair_kernel(const __grid
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(ACC_FULL + i), 1);
-      mbar_init(bar(ACC_EMPTY + i), 2 * kGemmEpiWarps);  // epilogue warps of both CTAs (used in the leader)
+      mbar_init(bar(ACC_EMPTY + i), 2 * C::EPI_WARPS);  // epilogue warps of both CTAs (used in the leader)
     }
     mbar_init(bar(DRAIN), 1);
+    for (int i = 0; i < C::EPI_WARPS; ++i) mbar_init(bar(RES + i), 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&p.tma_a);
@@ -308,157 +348,136 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_pair_kernel(const __grid
     }
   } else {
     // -------------------------------------------------------------- epilogue (both CTAs)
-    const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;  // TMEM lane quarter, column half
+    const int ew = warp - 2, quarter = warp & 3, chunk = ew >> 2;  // TMEM lane quarter, 64-column chunk
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t acc_empty0 = mapa_shared(bar(ACC_EMPTY), 0);
-    uint8_t* stg = smem + C::OFF_STG + ew * 2 * C::STG;
+    uint8_t* stg = smem + C::OFF_STG + ew * C::STG;
     float* bias_s = reinterpret_cast<float*>(smem + C::OFF_BIAS) + ew * 64;
     const long long nb = pack_blocks(p.N);
-    int sbuf = 0;  // staging buffer of the next chunk
-    uint32_t lt = 0;
+    uint32_t lt = 0, res_n = 0;
     for (Segments s(p, pair, pairs); s.next(); ++lt) {
       const int buf = lt & 1;
       const int m0 = (s.t / p.tiles_n) * 256 + 128 * static_cast<int>(rank) + quarter * 32;
-      const int n0 = (s.t % p.tiles_n) * BN + half * (BN / 2);
+      const int n = (s.t % p.tiles_n) * BN + chunk * 64;
       const long long row = m0 + lane;
       const bool in_row = row < p.M;
-      const bool ok = gemm_wait(bar(ACC_FULL + buf), (lt >> 1) & 1, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x74);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      const uint32_t acc = lane_base + buf * 256u + half * (BN / 2);
-#pragma unroll 1
-      for (int ch = 0; ch < C::CHUNKS; ++ch) {
-        const int n = n0 + 64 * ch;
-        const bool last = ch == C::CHUNKS - 1;
-        if (!s.whole()) {
-          // a part of a tile: fp32 sums into the pair's slot
-          float* dst = p.partial + ((static_cast<size_t>(2 * pair + (s.k0 ? 0 : 1)) * 256 + 128 * rank + quarter * 32 +
-                                     lane) * BN + half * (BN / 2) + 64 * ch);
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v[32];
-            tmem_ld32(acc + 64 * ch + 32 * h, v);
-            tmem_ld_wait();
-            if (in_row && n + 32 * h < p.N) {
-#pragma unroll
-              for (int c = 0; c < 8; ++c)
-                reinterpret_cast<uint4*>(dst + 32 * h)[c] = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-            }
-          }
-          if (last) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * buf);
-          }
-          continue;
-        }
-        if (n < p.N) {
-          if (p.bias) {
-            __syncwarp();
-            bias_s[lane] = n + lane < p.N ? elem_f32<T>(static_cast<const T*>(p.bias)[n + lane]) : 0.f;
-            bias_s[32 + lane] = n + 32 + lane < p.N ? elem_f32<T>(static_cast<const T*>(p.bias)[n + 32 + lane]) : 0.f;
-          }
-          // the staging buffers this chunk writes: the TMA stores that read them are done
-          if (lane == 0) {
-            if (p.z) bulk_wait_read_all();
-            else bulk_wait_read_but_one();
-          }
-          __syncwarp();
-        }
-        uint8_t* out_s = stg + (p.z ? 1 : sbuf) * C::STG;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const int c0 = n + 32 * h;
-          uint4 rr[4];
-          if (p.res && p.res_vec && in_row && c0 < p.N) {
-            const T* rp = static_cast<const T*>(p.res) + row * p.res_stride + c0;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              rr[c] = c0 + 8 * c < p.N ? *reinterpret_cast<const uint4*>(rp + 8 * c) : make_uint4(0, 0, 0, 0);
-          }
-          uint32_t raw[32];
-          tmem_ld32(acc + 64 * ch + 32 * h, raw);
-          tmem_ld_wait();
-          if (last && h == 1) {  // this warp's last read of the accumulator
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * buf);
-          }
-          if (c0 >= p.N) continue;
-          float v[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
-          if (p.bias) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 b = reinterpret_cast<const float4*>(bias_s + 32 * h)[i];
-              v[4 * i] += b.x;
-              v[4 * i + 1] += b.y;
-              v[4 * i + 2] += b.z;
-              v[4 * i + 3] += b.w;
-            }
-          }
-          if (p.z) stage32<T>(stg, lane, h, v);
-          if (p.z_codes) {
-            // (columns past N hold zeros: W's rows there are read as zeros, the bias too)
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) m = max(m, abs_bits(v[i]));
-            const uint32_t sc = pack_scale(m);
-            const float inv = pack_inv(sc), lim = pack_limit(sc);
-            if (in_row) {
-              uint4* dst = reinterpret_cast<uint4*>(p.z_codes + (row * nb + c0 / 32) * kPackBlock);
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                uint4 w;
-                w.x = pack_code4(v[16 * c], v[16 * c + 1], v[16 * c + 2], v[16 * c + 3], inv, lim);
-                w.y = pack_code4(v[16 * c + 4], v[16 * c + 5], v[16 * c + 6], v[16 * c + 7], inv, lim);
-                w.z = pack_code4(v[16 * c + 8], v[16 * c + 9], v[16 * c + 10], v[16 * c + 11], inv, lim);
-                w.w = pack_code4(v[16 * c + 12], v[16 * c + 13], v[16 * c + 14], v[16 * c + 15], inv, lim);
-                dst[c] = w;
-              }
-              p.z_scales[row * nb + c0 / 32] = static_cast<uint8_t>(sc);
-            }
-          }
-          act_any(p.act, v);
-          if (p.res && in_row) {
-            if (p.res_vec) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                float f[8];
-                unpack8<T>(rr[c], f);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[8 * c + e] += f[e];
-              }
-            } else {
-              const T* rp = static_cast<const T*>(p.res) + row * p.res_stride + c0;
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (c0 + i < p.N) v[i] += elem_f32<T>(rp[i]);
-            }
-          }
-          stage32<T>(out_s, lane, h, v);
-        }
-        if (n >= p.N) continue;
-        fence_proxy_async_smem();  // staging writes visible to the TMA stores
+      const bool work = n < p.N && m0 < p.M;  // anything to write (the same for the warp)
+      const bool whole = s.whole();
+      const bool res_ahead = p.res_tma && work && whole;
+      if (p.bias && work && whole) {
         __syncwarp();
-        if (lane == 0 && m0 < p.M) {
-          if (p.z && p.z_tma) tma_store_2d(&p.tma_z, smem_u32(stg), n, m0);
-          if (p.out_tma) tma_store_2d(&p.tma_out, smem_u32(out_s), n, m0);
-        }
-        if (lane == 0) bulk_commit_group();
-        if (p.z && !p.z_tma) {
-          if (p.z_w == 4) store_chunk_w<4>(stg, lane, p.z, p.z_stride, m0, n, p.M, p.N);
-          else if (p.z_w == 2) store_chunk_w<2>(stg, lane, p.z, p.z_stride, m0, n, p.M, p.N);
-          else store_chunk_w<1>(stg, lane, p.z, p.z_stride, m0, n, p.M, p.N);
-        }
-        if (!p.out_tma) {
-          if (p.out_w == 4) store_chunk_w<4>(out_s, lane, p.out, p.out_stride, m0, n, p.M, p.N);
-          else if (p.out_w == 2) store_chunk_w<2>(out_s, lane, p.out, p.out_stride, m0, n, p.M, p.N);
-          else store_chunk_w<1>(out_s, lane, p.out, p.out_stride, m0, n, p.M, p.N);
-        }
-        sbuf ^= 1;
+        bias_s[lane] = n + lane < p.N ? elem_f32<T>(static_cast<const T*>(p.bias)[n + lane]) : 0.f;
+        bias_s[32 + lane] = n + 32 + lane < p.N ? elem_f32<T>(static_cast<const T*>(p.bias)[n + 32 + lane]) : 0.f;
+        __syncwarp();
       }
+      if (res_ahead && lane == 0) {  // the residual chunk arrives in the staging while the main loop runs
+        bulk_wait_read_all();
+        fence_proxy_async_smem();  // after the warp's own reads of the staging (a __syncwarp ago)
+        mbar_arrive_expect_tx(bar(RES + ew), C::STG);
+        tma_load_2d(smem_u32(stg), &p.tma_res, bar(RES + ew), n, m0);
+      }
+      const bool ok = gemm_wait(bar(ACC_FULL + buf), (lt >> 1) & 1, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x74);
+      bool res_ok = true;
+      if (res_ahead) {
+        res_ok = gemm_wait(bar(RES + ew), res_n & 1, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x75);
+        if (!res_ok) gemm_drain(bar(RES + ew), res_n & 1, p.wait_limit_ns);
+        ++res_n;
+      }
+      if (!__all_sync(0xffffffffu, ok && res_ok)) break;
+      tc_fence_after();
+      const uint32_t acc = lane_base + buf * 256u + chunk * 64;
+      auto release = [&] {  // this warp's last read of the accumulator is done
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * buf);
+      };
+      auto load = [&](int h, float (&v)[32]) {
+        uint32_t (&raw)[32] = reinterpret_cast<uint32_t (&)[32]>(v);
+        tmem_ld32(acc + 32 * h, raw);
+        tmem_ld_wait();
+      };
+      if (!work) {
+        release();
+        continue;
+      }
+      const int halves = n + 32 < p.N ? 2 : 1;
+      if (!whole) {  // a part of a tile: fp32 sums into the pair's slot
+        float* dst = p.partial + (static_cast<size_t>(2 * pair + (s.k0 ? 0 : 1)) * 256 + 128 * rank + quarter * 32 + lane) * BN +
+                     chunk * 64;
+#pragma unroll 1
+        for (int h = 0; h < halves; ++h) {
+          float v[32];
+          load(h, v);
+          if (in_row) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              reinterpret_cast<float4*>(dst + 32 * h)[c] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+          }
+        }
+        release();
+        continue;
+      }
+      if (p.z) {  // the accumulator is read once more below: cheaper than holding it
+        staging_free(lane);
+#pragma unroll 1
+        for (int h = 0; h < halves; ++h) {
+          float v[32];
+          load(h, v);
+          if (p.bias) add_bias(v, bias_s + 32 * h);
+          stage32<T>(stg, lane, h, v);
+        }
+        store_staged(&p.tma_z, p.z_tma, p.z_w, stg, lane, p.z, p.z_stride, m0, n, p.M, p.N);
+      }
+      if (p.z_codes) {
+        // (columns past N hold zeros: W's rows there are read as zeros, the bias too)
+        staging_free(lane);
+#pragma unroll 1
+        for (int h = 0; h < halves; ++h) {
+          float v[32];
+          load(h, v);
+          if (p.bias) add_bias(v, bias_s + 32 * h);
+          uint32_t codes[8];
+          const uint32_t sc = pack32(v, codes);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint4 w = make_uint4(codes[4 * c], codes[4 * c + 1], codes[4 * c + 2], codes[4 * c + 3]);
+            // rows of 64 bytes, 64-byte swizzle
+            *reinterpret_cast<uint4*>(stg + lane * 64 + (((2 * h + c) ^ ((lane >> 1) & 3)) << 4)) = w;
+          }
+          if (in_row) p.z_scales[row * nb + n / 32 + h] = static_cast<uint8_t>(sc);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&p.tma_codes, smem_u32(stg), n, m0);
+          bulk_commit_group();
+        }
+      }
+      if (!res_ahead) staging_free(lane);
+#pragma unroll 1
+      for (int h = 0; h < halves; ++h) {
+        float v[32];
+        load(h, v);
+        if (h == halves - 1) release();
+        if (p.bias) add_bias(v, bias_s + 32 * h);
+        act_any(p.act, v);
+        if (res_ahead) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float f[8];
+            unpack8<T>(*stage_part(stg, lane, 4 * h + c), f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[8 * c + e] += f[e];
+          }
+        } else if (p.res && in_row) {
+          const T* rp = static_cast<const T*>(p.res) + row * p.res_stride + n + 32 * h;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (n + 32 * h + i < p.N) v[i] += elem_f32<T>(rp[i]);
+        }
+        stage32<T>(stg, lane, h, v);
+      }
+      store_staged(&p.tma_out, p.out_tma, p.out_w, stg, lane, p.out, p.out_stride, m0, n, p.M, p.N);
     }
     if (lane == 0) bulk_wait_all();  // output written before the CTA ends
   }
@@ -575,6 +594,20 @@ int encode_map(CUtensorMap* m, const void* base, long long cols, long long rows,
   return r == CUDA_SUCCESS ? 0 : FRATTN_E_TMAP;
 }
 
+// Codes of a checkpoint: rows of 32 nb bytes.
+int encode_codes_map(CUtensorMap* m, const void* base, long long cols, long long rows) {
+  const TmapEncodeFn enc = tmap_encoder();
+  if (!enc) return FRATTN_E_TMAP;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols)};
+  cuuint32_t box[2] = {64, 32};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : FRATTN_E_TMAP;
+}
+
 bool rows16(const void* p, long long stride) { return aligned_to(p, 16) && stride % 8 == 0; }
 
 int sm_pairs() {
@@ -607,7 +640,7 @@ GemmPlan gemm_plan(int M, int N, int nk) {
     const long long total = tiles * nk;
     int split = static_cast<int>((total + P - 1) / P);
     if (split < 4) split = 4;
-    if (split < nk && tiles % P != 0) {
+    if (tiles % P != 0) {
       const int pairs = static_cast<int>((total + split - 1) / split);
       const double rows = M < 256 ? M : 256;
       const double us = split * step_us + 6.0 + 2.0 * pairs * rows * bn * 4 * 2 / 4e6;
@@ -640,7 +673,7 @@ int gemm_launch(GemmParams& p, const GemmPlan& plan, cudaStream_t st) {
   attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(2 * plan.pairs);
-  lc.blockDim = dim3(kGemmThreads);
+  lc.blockDim = dim3(C::THREADS);
   lc.dynamicSmemBytes = C::SMEM;
   lc.stream = st;
   lc.attrs = &attr;
@@ -684,8 +717,9 @@ int gemm(GemmParams& p, const Mat& a, const Mat& b, int M, int N, int K, void* w
     p.z_w = width(p.z, p.z_stride);
     if (p.z_tma && encode_map(&p.tma_z, p.z, N, M, p.z_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
   }
-  // (a vector of 8 may then start inside the row and end past it: only where N % 8 == 0)
-  p.res_vec = p.res && rows16(p.res, p.res_stride) && N % 8 == 0;
+  if (p.z_codes && encode_codes_map(&p.tma_codes, p.z_codes, pack_blocks(N) * kPackBlock, M)) return FRATTN_E_TMAP;
+  p.res_tma = p.res && rows16(p.res, p.res_stride) && p.res_stride >= N && !p.z && !p.z_codes;
+  if (p.res_tma && encode_map(&p.tma_res, p.res, N, M, p.res_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
   if (plan.bn == 256) return gemm_launch<256, AMN, BMN, T>(p, plan, st);
   return gemm_launch<128, AMN, BMN, T>(p, plan, st);
 }
