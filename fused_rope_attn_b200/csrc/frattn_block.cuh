@@ -31,6 +31,8 @@ __device__ __forceinline__ __half f32_elem<__half>(float x) { return __float2hal
 template <int BYTES>
 struct RawVec;
 template <>
+struct RawVec<1> { using type = uint8_t; };
+template <>
 struct RawVec<2> { using type = uint16_t; };
 template <>
 struct RawVec<4> { using type = uint32_t; };
@@ -39,29 +41,72 @@ struct RawVec<8> { using type = uint2; };
 template <>
 struct RawVec<16> { using type = uint4; };
 
-// VEC elements as raw words (loads of several vectors can be in flight before
-// any of them is converted).
+__device__ __forceinline__ void raw_words(uint16_t r, uint32_t* w) { w[0] = r; }
+__device__ __forceinline__ void raw_words(uint8_t r, uint32_t* w) { w[0] = r; }
+__device__ __forceinline__ void raw_words(uint32_t r, uint32_t* w) { w[0] = r; }
+__device__ __forceinline__ void raw_words(uint2 r, uint32_t* w) { w[0] = r.x; w[1] = r.y; }
+__device__ __forceinline__ void raw_words(uint4 r, uint32_t* w) { w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w; }
+
+// VEC elements as 32-bit words, as loaded (loads of several vectors can be in flight
+// before any of them is converted; element-sized pieces would each take a register).
 template <typename T, int VEC>
 struct Vec {
   static constexpr int kBytes = VEC * static_cast<int>(sizeof(T));
   static constexpr int kPart = kBytes > 16 ? 16 : kBytes;
   static constexpr int kParts = kBytes / kPart;
+  static constexpr int kPartWords = kPart < 4 ? 1 : kPart / 4;
   using Raw = typename RawVec<kPart>::type;
-  union {
-    Raw raw[kParts];
-    T elem[VEC];
-  };
-  __device__ __forceinline__ Vec() {}
+  uint32_t w[kParts * kPartWords];
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) raw[i] = __ldg(reinterpret_cast<const Raw*>(p) + i);
+    for (int i = 0; i < kParts; ++i) raw_words(__ldg(reinterpret_cast<const Raw*>(p) + i), w + i * kPartWords);
   }
-  __device__ __forceinline__ void store(T* p) const {
+  __device__ __forceinline__ void get(float (&v)[VEC]) const {
+    if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) reinterpret_cast<Raw*>(p)[i] = raw[i];
+      for (int i = 0; i < VEC; ++i) v[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const __half2 h = *reinterpret_cast<const __half2*>(&w[i / 2]);
+        v[i] = i & 1 ? __high2float(h) : __low2float(h);
+      }
+    }
   }
-  __device__ __forceinline__ float get(int i) const { return elem_f32<T>(elem[i]); }
-  __device__ __forceinline__ void set(int i, float x) { elem[i] = f32_elem<T>(x); }
+  // v rounded to T, to p
+  static __device__ __forceinline__ void put(T* p, const float (&v)[VEC]) {
+    if constexpr (std::is_same<T, float>::value) {
+      if constexpr (VEC == 1) p[0] = v[0];
+      else
+#pragma unroll
+        for (int i = 0; i < VEC / 4; ++i)
+          reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else if constexpr (VEC == 1) {
+      p[0] = f32_elem<T>(v[0]);
+    } else if constexpr (VEC == 4) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    } else {
+      *reinterpret_cast<uint4*>(p) =
+          make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    }
+  }
+};
+
+// VEC int8 codes of a checkpoint, as loaded.
+template <int VEC>
+struct CodeVec {
+  static constexpr int kWords = VEC < 4 ? 1 : VEC / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const int8_t* p) {
+    raw_words(__ldg(reinterpret_cast<const typename RawVec<VEC>::type*>(p)), w);
+  }
+  __device__ __forceinline__ void get(float step, float (&v)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i & 3)))) * step;
+  }
 };
 
 // Largest vector width of {8, 4, 1} elements of esz bytes that every listed

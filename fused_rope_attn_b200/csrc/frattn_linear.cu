@@ -756,10 +756,7 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
   const long long step = gridDim.y;
   for (long long row0 = blockIdx.y; row0 < p.T; row0 += step * R) {
     Vec<T, VEC> dy[R], z[R];
-    union {
-      typename RawVec<VEC == 1 ? 2 : VEC>::type raw;
-      int8_t c[VEC == 1 ? 2 : VEC];
-    } q[R];
+    CodeVec<VEC> q[R];
     uint32_t scale[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -768,9 +765,7 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
         dy[r].load(static_cast<const T*>(p.dout) + row * p.dout_stride + c);
         if constexpr (ACT != FRATTN_ACT_NONE) {
           if constexpr (PACKED) {
-            const int8_t* src = p.z_codes + row * nb * kPackBlock + c;
-            if constexpr (VEC == 1) q[r].c[0] = __ldg(src);
-            else q[r].raw = __ldg(reinterpret_cast<const typename RawVec<VEC>::type*>(src));
+            q[r].load(p.z_codes + row * nb * kPackBlock + c);
             scale[r] = __ldg(p.z_scales + row * nb + v * VEC / kPackBlock);
           } else {
             z[r].load(static_cast<const T*>(p.z) + row * p.z_stride + c);
@@ -782,17 +777,18 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + r * step;
       if (row >= p.T) break;
-      const float st = PACKED && ACT != FRATTN_ACT_NONE ? pack_step(scale[r]) : 0.f;
-      Vec<T, VEC> o;
+      float d[VEC];
+      dy[r].get(d);
+      if constexpr (ACT != FRATTN_ACT_NONE) {
+        float f[VEC];
+        if constexpr (PACKED) q[r].get(pack_step(scale[r]), f);
+        else z[r].get(f);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float d = dy[r].get(e);
-        if constexpr (ACT != FRATTN_ACT_NONE)
-          d *= act_grad_f<ACT>(PACKED ? static_cast<float>(q[r].c[e]) * st : z[r].get(e));
-        sum[e] += d;
-        o.set(e, d);
+        for (int e = 0; e < VEC; ++e) d[e] *= act_grad_f<ACT>(f[e]);
       }
-      if (p.dz) o.store(static_cast<T*>(p.dz) + row * p.dz_stride + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[e] += d[e];
+      if (p.dz) Vec<T, VEC>::put(static_cast<T*>(p.dz) + row * p.dz_stride + c, d);
     }
   }
   if (p.partial) {

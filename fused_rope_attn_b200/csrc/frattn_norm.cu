@@ -9,10 +9,10 @@
 // All sums are kept in 32 bits; the variance is the sum of squared differences
 // from the mean over values held in registers (no difference of large sums).
 //
-// Both are bound by the bytes of the rows. One block holds R whole rows in
-// registers (one vector of up to 8 columns per thread for rows of up to 8192
-// columns), so every row is read once; R = 4 rows share each block-wide
-// reduction's barrier and keep four rows' loads in flight. The weight
+// Both are bound by the bytes of the rows. A block holds R whole rows in registers
+// (one vector of up to 8 columns per thread for rows of up to 8192 columns), so every
+// row is read once; the next R rows' loads are issued before the current ones are
+// worked on, and R rows share each block-wide reduction's barrier. The weight
 // gradients stay in the registers of the thread that owns the column over all
 // rows of a block; each block writes one partial row, and column_finish adds
 // the partial rows in a fixed order (no atomics: the same bits every run).
@@ -28,6 +28,7 @@ struct NormParams {
   const void* w;        // [C] or null (ones)
   const void* b;        // [C] or null (zeros), forward only
   int w_f32;            // w, b, dw, db are fp32 (else the element type)
+  int w_vec;            // w and b are 16-byte aligned
   const void* dy;       // [T, C] rows of dy_stride elements, backward only
   long long dy_stride;
   void* out;            // y or dx
@@ -41,89 +42,123 @@ struct NormParams {
 
 namespace {
 
-// Sums over the block's threads of R values; every thread gets them. `red` holds
-// R x 32 floats and must not be reused before the next barrier but one.
+// Sums over the block's threads of R values (a power of two); every thread gets them.
+// Within a warp the lanes split the values among them as they halve: R - 1 + 5 - log2 R
+// shuffles instead of 5 R. `red` holds 32 R floats and must not be reused before the
+// next barrier but one.
 template <int R>
 __device__ __forceinline__ void block_sum(float (&s)[R], float* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  float t[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int r = 0; r < R; ++r) t[r] = s[r];
+  int o = 16;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
-  const int nw = blockDim.x >> 5;
-  if (nw == 1) return;
-  const int warp = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) {
+  for (int n = R; n > 1; n >>= 1, o >>= 1) {
+    const bool up = lane & o;  // this lane keeps the upper half of the values
 #pragma unroll
-    for (int r = 0; r < R; ++r) red[r * 32 + warp] = s[r];
+    for (int r = 0; r < n / 2; ++r) {
+      const float give = up ? t[r] : t[r + n / 2], keep = up ? t[r + n / 2] : t[r];
+      t[r] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
   }
+#pragma unroll
+  for (int q = 16 / R; q > 0; q >>= 1) t[0] += __shfl_xor_sync(0xffffffffu, t[0], q);
+  // value r now lies in the lanes whose bits 4 .. 5 - log2 R spell r (highest bit first)
+  if (nw == 1) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] = __shfl_sync(0xffffffffu, t[0], r * (32 / R));
+    return;
+  }
+  if (lane % (32 / R) == 0) red[warp * R + lane / (32 / R)] = t[0];
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    float t = 0.f;
-    for (int w = 0; w < nw; ++w) t += red[r * 32 + w];
-    s[r] = t;
+  for (int r = 0; r < R; ++r) s[r] = 0.f;
+  for (int w = 0; w < nw; ++w) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] += red[w * R + r];
   }
 }
 
 // Parameter vector (weight or bias) of columns [c, c + VEC) in 32 bits.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_param(const void* p, int f32, int c, float fill, float (&v)[VEC]) {
+__device__ __forceinline__ void load_param(const void* p, int f32, int vec, int c, float fill, float (&v)[VEC]) {
+  if (!p) {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    if (!p) v[e] = fill;
-    else v[e] = f32 ? __ldg(static_cast<const float*>(p) + c + e) : elem_f32<T>(static_cast<const T*>(p)[c + e]);
+    for (int e = 0; e < VEC; ++e) v[e] = fill;
+  } else if (vec) {
+    if (f32) {
+      Vec<float, VEC> x;
+      x.load(static_cast<const float*>(p) + c);
+      x.get(v);
+    } else {
+      Vec<T, VEC> x;
+      x.load(static_cast<const T*>(p) + c);
+      x.get(v);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      v[e] = f32 ? __ldg(static_cast<const float*>(p) + c + e) : elem_f32<T>(static_cast<const T*>(p)[c + e]);
   }
 }
 
 template <typename T, int VEC, int NV, int R>
-__global__ void __launch_bounds__(R == 1 ? 1024 : 512) layer_norm_fwd_kernel(const NormParams p) {
-  __shared__ float red[2][R * 32];
+__global__ void __launch_bounds__(R == 1 ? 1024 : R == 2 ? 512 : 256) layer_norm_fwd_kernel(const NormParams p) {
+  __shared__ __align__(16) float red[2][R * 32];
   const int nvec = p.C / VEC;
   float w[NV][VEC], b[NV][VEC];
+  bool has[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    if (v < nvec) {
-      load_param<T, VEC>(p.w, p.w_f32, v * VEC, 1.f, w[i]);
-      load_param<T, VEC>(p.b, p.w_f32, v * VEC, 0.f, b[i]);
+    has[i] = v < nvec;
+    if (has[i]) {
+      load_param<T, VEC>(p.w, p.w_f32, p.w_vec, v * VEC, 1.f, w[i]);
+      load_param<T, VEC>(p.b, p.w_f32, p.w_vec, v * VEC, 0.f, b[i]);
     }
   }
   const float inv_c = 1.f / static_cast<float>(p.C);
-  for (long long row0 = static_cast<long long>(blockIdx.x) * R; row0 < p.T; row0 += static_cast<long long>(gridDim.x) * R) {
-    Vec<T, VEC> x[R][NV];
-    float s[R];
+  const long long step = static_cast<long long>(gridDim.x) * R;
+  Vec<T, VEC> next[R][NV];
+  auto fetch = [&](long long row0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const T* row = static_cast<const T*>(p.x) + (row0 + r) * p.x_stride;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v < nvec && row0 + r < p.T) x[r][i].load(row + static_cast<size_t>(v) * VEC);
-      }
+      for (int i = 0; i < NV; ++i)
+        if (has[i] && row0 + r < p.T) next[r][i].load(row + static_cast<size_t>(threadIdx.x + i * blockDim.x) * VEC);
     }
+  };
+  long long row0 = static_cast<long long>(blockIdx.x) * R;
+  fetch(row0);
+  for (; row0 < p.T; row0 += step) {
+    float x[R][NV][VEC], s[R], mean[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       s[r] = 0.f;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (static_cast<int>(threadIdx.x + i * blockDim.x) < nvec && row0 + r < p.T) {
+      for (int i = 0; i < NV; ++i) {
+        next[r][i].get(x[r][i]);
+        if (has[i]) {  // (rows past the last hold what an earlier pass left there, and go nowhere)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) s[r] += x[r][i].get(e);
+          for (int e = 0; e < VEC; ++e) s[r] += x[r][i][e];
         }
+      }
     }
+    fetch(row0 + step);
     block_sum<R>(s, red[0]);
-    float mean[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       mean[r] = s[r] * inv_c;
       s[r] = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (static_cast<int>(threadIdx.x + i * blockDim.x) < nvec && row0 + r < p.T) {
+        if (has[i]) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            const float d = x[r][i].get(e) - mean[r];
-            s[r] += d * d;
+            x[r][i][e] -= mean[r];
+            s[r] += x[r][i][e] * x[r][i][e];
           }
         }
     }
@@ -139,15 +174,13 @@ __global__ void __launch_bounds__(R == 1 ? 1024 : 512) layer_norm_fwd_kernel(con
       }
       T* out = static_cast<T*>(p.out) + row * p.out_stride;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v < nvec) {
-          Vec<T, VEC> y;
+      for (int i = 0; i < NV; ++i)
+        if (has[i]) {
+          float y[VEC];
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) y.set(e, (x[r][i].get(e) - mean[r]) * rstd * w[i][e] + b[i][e]);
-          y.store(out + static_cast<size_t>(v) * VEC);
+          for (int e = 0; e < VEC; ++e) y[e] = x[r][i][e] * rstd * w[i][e] + b[i][e];
+          Vec<T, VEC>::put(out + static_cast<size_t>(threadIdx.x + i * blockDim.x) * VEC, y);
         }
-      }
     }
   }
 }
@@ -178,8 +211,8 @@ __global__ void __launch_bounds__(1024) layer_norm_fwd_wide_kernel(const NormPar
     }
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
       float w[1], b[1];
-      load_param<T, 1>(p.w, p.w_f32, c, 1.f, w);
-      load_param<T, 1>(p.b, p.w_f32, c, 0.f, b);
+      load_param<T, 1>(p.w, p.w_f32, 0, c, 1.f, w);
+      load_param<T, 1>(p.b, p.w_f32, 0, c, 0.f, b);
       out[c] = f32_elem<T>((elem_f32<T>(x[c]) - mean) * rstd * w[0] + b[0]);
     }
   }
@@ -192,76 +225,85 @@ struct NormIn {
   __device__ __forceinline__ void load(const NormParams& p, long long row, int vec) {
     v.load(static_cast<const T*>(p.x) + row * p.x_stride + static_cast<size_t>(vec) * VEC);
   }
-  __device__ __forceinline__ float get(int e) const { return v.get(e); }
+  __device__ __forceinline__ void get(float (&f)[VEC]) const { v.get(f); }
 };
 template <typename T, int VEC>
 struct NormIn<T, VEC, true> {
-  union {
-    typename RawVec<VEC == 1 ? 2 : VEC>::type raw;
-    int8_t c[VEC == 1 ? 2 : VEC];
-  };
+  CodeVec<VEC> c;
   uint32_t scale;
-  __device__ __forceinline__ NormIn() {}
   __device__ __forceinline__ void load(const NormParams& p, long long row, int vec) {
     const long long nb = pack_blocks(p.C);
-    const int8_t* src = p.codes + row * nb * kPackBlock + static_cast<size_t>(vec) * VEC;
-    if constexpr (VEC == 1) c[0] = __ldg(src);
-    else raw = __ldg(reinterpret_cast<const typename RawVec<VEC>::type*>(src));
+    c.load(p.codes + row * nb * kPackBlock + static_cast<size_t>(vec) * VEC);
     scale = __ldg(p.scales + row * nb + vec * VEC / kPackBlock);
   }
-  __device__ __forceinline__ float get(int e) const { return static_cast<float>(c[e]) * pack_step(scale); }
+  __device__ __forceinline__ void get(float (&f)[VEC]) const { c.get(pack_step(scale), f); }
 };
 
 template <typename T, int VEC, int NV, int R, bool PACKED>
-__global__ void __launch_bounds__(R == 1 ? 1024 : 512) layer_norm_bwd_kernel(const NormParams p) {
-  __shared__ float red[2][2 * R * 32];
+__global__ void __launch_bounds__(R == 1 ? 1024 : R == 2 ? 512 : 256) layer_norm_bwd_kernel(const NormParams p) {
+  __shared__ __align__(16) float red[2][2 * R * 32];
   const int nvec = p.C / VEC;
   float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
+  bool has[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    if (v < nvec) load_param<T, VEC>(p.w, p.w_f32, v * VEC, 1.f, w[i]);
+    has[i] = v < nvec;
+    if (has[i]) load_param<T, VEC>(p.w, p.w_f32, p.w_vec, v * VEC, 1.f, w[i]);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dw[i][e] = db[i][e] = 0.f;
   }
   const float inv_c = 1.f / static_cast<float>(p.C);
-  int phase = 0;
-  for (long long row0 = static_cast<long long>(blockIdx.x) * R; row0 < p.T;
-       row0 += static_cast<long long>(gridDim.x) * R, phase ^= 1) {
-    NormIn<T, VEC, PACKED> x[R][NV];
-    Vec<T, VEC> dy[R][NV];
-    float mean[R], rstd[R], s[2 * R];
+  const long long step = static_cast<long long>(gridDim.x) * R;
+  NormIn<T, VEC, PACKED> nx[R][NV];
+  Vec<T, VEC> ny[R][NV];
+  float nmean[R], nrstd[R];
+  auto fetch = [&](long long row0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + r;
-      const bool in = row < p.T;
-      mean[r] = in ? __ldg(p.mean + row) : 0.f;
-      rstd[r] = in ? __ldg(p.rstd + row) : 0.f;
+      nmean[r] = nrstd[r] = 0.f;
+      if (row < p.T) {
+        nmean[r] = __ldg(p.mean + row);
+        nrstd[r] = __ldg(p.rstd + row);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v < nvec && in) {
-          x[r][i].load(p, row, v);
-          dy[r][i].load(static_cast<const T*>(p.dy) + row * p.dy_stride + static_cast<size_t>(v) * VEC);
+        for (int i = 0; i < NV; ++i) {
+          const int v = threadIdx.x + i * blockDim.x;
+          if (has[i]) {
+            nx[r][i].load(p, row, v);
+            ny[r][i].load(static_cast<const T*>(p.dy) + row * p.dy_stride + static_cast<size_t>(v) * VEC);
+          }
         }
       }
     }
+  };
+  int phase = 0;
+  long long row0 = static_cast<long long>(blockIdx.x) * R;
+  fetch(row0);
+  for (; row0 < p.T; row0 += step, phase ^= 1) {
+    float h[R][NV][VEC], d[R][NV][VEC], rstd[R], s[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       s[2 * r] = s[2 * r + 1] = 0.f;
+      rstd[r] = nrstd[r];
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (static_cast<int>(threadIdx.x + i * blockDim.x) < nvec && row0 + r < p.T) {
+        if (has[i] && row0 + r < p.T) {
+          nx[r][i].get(h[r][i]);
+          ny[r][i].get(d[r][i]);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            const float d = dy[r][i].get(e), h = (x[r][i].get(e) - mean[r]) * rstd[r], g = d * w[i][e];
+            const float y = d[r][i][e], t = (h[r][i][e] - nmean[r]) * rstd[r], g = y * w[i][e];
+            dw[i][e] += y * t;
+            db[i][e] += y;
             s[2 * r] += g;
-            s[2 * r + 1] += g * h;
-            dw[i][e] += d * h;
-            db[i][e] += d;
+            s[2 * r + 1] += g * t;
+            h[r][i][e] = t;
+            d[r][i][e] = g;
           }
         }
     }
+    fetch(row0 + step);
     block_sum<2 * R>(s, red[phase]);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -270,18 +312,13 @@ __global__ void __launch_bounds__(R == 1 ? 1024 : 512) layer_norm_bwd_kernel(con
       const float c1 = s[2 * r] * inv_c, c2 = s[2 * r + 1] * inv_c;
       T* out = static_cast<T*>(p.out) + row * p.out_stride;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v < nvec) {
-          Vec<T, VEC> o;
+      for (int i = 0; i < NV; ++i)
+        if (has[i]) {
+          float o[VEC];
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float h = (x[r][i].get(e) - mean[r]) * rstd[r];
-            o.set(e, rstd[r] * (dy[r][i].get(e) * w[i][e] - c1 - h * c2));
-          }
-          o.store(out + static_cast<size_t>(v) * VEC);
+          for (int e = 0; e < VEC; ++e) o[e] = rstd[r] * (d[r][i][e] - c1 - h[r][i][e] * c2);
+          Vec<T, VEC>::put(out + static_cast<size_t>(threadIdx.x + i * blockDim.x) * VEC, o);
         }
-      }
     }
   }
   if (p.partial) {
@@ -289,7 +326,7 @@ __global__ void __launch_bounds__(R == 1 ? 1024 : 512) layer_norm_bwd_kernel(con
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = threadIdx.x + i * blockDim.x;
-      if (v < nvec) {
+      if (has[i]) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           mine[static_cast<size_t>(v) * VEC + e] = dw[i][e];
@@ -314,21 +351,25 @@ __global__ void __launch_bounds__(1024) layer_norm_bwd_wide_kernel(const NormPar
     float s[2] = {0.f, 0.f};
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
       float w[1];
-      load_param<T, 1>(p.w, p.w_f32, c, 1.f, w);
-      NormIn<T, 1, PACKED> x;
-      x.load(p, row, c);
+      load_param<T, 1>(p.w, p.w_f32, 0, c, 1.f, w);
+      NormIn<T, 1, PACKED> in;
+      float x[1];
+      in.load(p, row, c);
+      in.get(x);
       const float g = elem_f32<T>(dy[c]) * w[0];
       s[0] += g;
-      s[1] += g * (x.get(0) - mean) * rstd;
+      s[1] += g * (x[0] - mean) * rstd;
     }
     block_sum<2>(s, red[phase]);
     const float c1 = s[0] * inv_c, c2 = s[1] * inv_c;
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
       float w[1];
-      load_param<T, 1>(p.w, p.w_f32, c, 1.f, w);
-      NormIn<T, 1, PACKED> x;
-      x.load(p, row, c);
-      out[c] = f32_elem<T>(rstd * (elem_f32<T>(dy[c]) * w[0] - c1 - (x.get(0) - mean) * rstd * c2));
+      load_param<T, 1>(p.w, p.w_f32, 0, c, 1.f, w);
+      NormIn<T, 1, PACKED> in;
+      float x[1];
+      in.load(p, row, c);
+      in.get(x);
+      out[c] = f32_elem<T>(rstd * (elem_f32<T>(dy[c]) * w[0] - c1 - (x[0] - mean) * rstd * c2));
     }
   }
 }
@@ -339,10 +380,12 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_wide_cols_kernel(const Nor
   if (c >= p.C) return;
   float dw = 0.f, db = 0.f;
   for (long long row = blockIdx.y; row < p.T; row += gridDim.y) {
-    NormIn<T, 1, PACKED> x;
-    x.load(p, row, c);
+    NormIn<T, 1, PACKED> in;
+    float x[1];
+    in.load(p, row, c);
+    in.get(x);
     const float d = elem_f32<T>(static_cast<const T*>(p.dy)[row * p.dy_stride + c]);
-    dw += d * (x.get(0) - __ldg(p.mean + row)) * __ldg(p.rstd + row);
+    dw += d * (x[0] - __ldg(p.mean + row)) * __ldg(p.rstd + row);
     db += d;
   }
   p.partial[static_cast<size_t>(blockIdx.y) * 2 * p.C + c] = dw;
@@ -350,7 +393,8 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_wide_cols_kernel(const Nor
 }
 
 // out_a[c] = sum over g < groups of partial[g][a][c], a < arrays: 32 columns and
-// 16 row lanes per block, the lanes' sums joined in a fixed order.
+// 32 row lanes per block, the lanes' sums joined in a fixed order. Launched while the
+// kernel that writes the partial rows still runs (programmatic dependent launch).
 struct FinishParams {
   const float* partial;
   int groups, arrays, C;
@@ -358,23 +402,27 @@ struct FinishParams {
   int dtype;  // of the outputs
 };
 
-__global__ void __launch_bounds__(512) column_finish_kernel(const FinishParams p) {
-  __shared__ float red[16][33];
+__global__ void __launch_bounds__(1024) column_finish_kernel(const FinishParams p) {
+  __shared__ float red[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x, a = blockIdx.y;
+  griddep_wait();
   float s = 0.f;
   if (c < p.C)
-#pragma unroll 4
-    for (int g = threadIdx.y; g < p.groups; g += 16)
-      s += __ldg(p.partial + (static_cast<size_t>(g) * p.arrays + a) * p.C + c);
+#pragma unroll 8
+    for (int g = threadIdx.y; g < p.groups; g += 32)
+      s += __ldcg(p.partial + (static_cast<size_t>(g) * p.arrays + a) * p.C + c);
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y || c >= p.C || !p.out[a]) return;
-  float t = 0.f;
+  // one warp per column: lane g holds row lane g's sum
+  s = red[threadIdx.x][threadIdx.y];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) t += red[i][threadIdx.x];
-  if (p.dtype == FRATTN_F32) static_cast<float*>(p.out[a])[c] = t;
-  else if (p.dtype == FRATTN_BF16) static_cast<__nv_bfloat16*>(p.out[a])[c] = __float2bfloat16_rn(t);
-  else static_cast<__half*>(p.out[a])[c] = __float2half_rn(t);
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int d = blockIdx.x * 32 + threadIdx.y;
+  void* out = a ? p.out[1] : p.out[0];
+  if (threadIdx.x || d >= p.C || !out) return;
+  if (p.dtype == FRATTN_F32) static_cast<float*>(out)[d] = s;
+  else if (p.dtype == FRATTN_BF16) static_cast<__nv_bfloat16*>(out)[d] = __float2bfloat16_rn(s);
+  else static_cast<__half*>(out)[d] = __float2half_rn(s);
 }
 
 // ---------------------------------------------------------------- checkpoints
@@ -411,24 +459,27 @@ __global__ void __launch_bounds__(256) act_pack_kernel(const PackParams p) {
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + r * step;
       uint32_t m = 0;
-      if (has && row < p.T) {
+      float f[VEC];
+      x[r].get(f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) m = max(m, abs_bits(x[r].get(e)));
+      for (int e = 0; e < VEC; ++e) {
+        if (!has) f[e] = 0.f;
+        m = max(m, abs_bits(f[e]));
       }
 #pragma unroll
       for (int o = G / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
       const uint32_t scale = pack_scale(m);
       const float inv = pack_inv(scale), lim = pack_limit(scale);
-      union {
-        typename RawVec<VEC == 1 ? 2 : VEC>::type raw;
-        int8_t c[VEC == 1 ? 2 : VEC];
-      } o;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) o.c[e] = has && row < p.T ? static_cast<int8_t>(pack_code(x[r].get(e), inv, lim)) : 0;
       if (in_row && row < p.T) {
         int8_t* dst = p.codes + row * nb * kPackBlock + static_cast<size_t>(v) * VEC;
-        if constexpr (VEC == 1) *dst = o.c[0];
-        else *reinterpret_cast<typename RawVec<VEC>::type*>(dst) = o.raw;
+        if constexpr (VEC == 1) {
+          *dst = static_cast<int8_t>(pack_code(f[0], inv, lim));
+        } else if constexpr (VEC == 4) {
+          *reinterpret_cast<uint32_t*>(dst) = pack_code4(f[0], f[1], f[2], f[3], inv, lim);
+        } else {
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack_code4(f[0], f[1], f[2], f[3], inv, lim),
+                                                      pack_code4(f[4], f[5], f[6], f[7], inv, lim));
+        }
         if (v % G == 0) p.scales[row * nb + v / G] = static_cast<uint8_t>(scale);
       }
     }
@@ -443,18 +494,13 @@ __global__ void __launch_bounds__(256) act_unpack_kernel(const PackParams p) {
   if (v * VEC >= p.C) return;
   const long long step = static_cast<long long>(gridDim.y) * blockDim.y;
   for (long long row0 = static_cast<long long>(blockIdx.y) * blockDim.y + threadIdx.y; row0 < p.T; row0 += step * R) {
-    union {
-      typename RawVec<VEC == 1 ? 2 : VEC>::type raw;
-      int8_t c[VEC == 1 ? 2 : VEC];
-    } in[R];
+    CodeVec<VEC> in[R];
     uint32_t scale[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + r * step;
       if (row < p.T) {
-        const int8_t* src = p.codes + row * nb * kPackBlock + static_cast<size_t>(v) * VEC;
-        if constexpr (VEC == 1) in[r].c[0] = __ldg(src);
-        else in[r].raw = __ldg(reinterpret_cast<const typename RawVec<VEC>::type*>(src));
+        in[r].load(p.codes + row * nb * kPackBlock + static_cast<size_t>(v) * VEC);
         scale[r] = __ldg(p.scales + row * nb + v * VEC / kPackBlock);
       }
     }
@@ -462,11 +508,9 @@ __global__ void __launch_bounds__(256) act_unpack_kernel(const PackParams p) {
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + r * step;
       if (row >= p.T) break;
-      const float st = pack_step(scale[r]);
-      Vec<T, VEC> o;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) o.set(e, static_cast<float>(in[r].c[e]) * st);
-      o.store(static_cast<T*>(p.out) + row * p.out_stride + static_cast<size_t>(v) * VEC);
+      float f[VEC];
+      in[r].get(pack_step(scale[r]), f);
+      Vec<T, VEC>::put(static_cast<T*>(p.out) + row * p.out_stride + static_cast<size_t>(v) * VEC, f);
     }
   }
 }
@@ -494,48 +538,73 @@ int with_shape(int vec, int C, F&& f) {
   return f(std::integral_constant<int, 1>(), std::integral_constant<int, 8>(), threads_for(nvec, 8));
 }
 
-// Rows per block pass: 4 when that still gives every SM a block and the block is
-// no larger than 512 threads, else 1 (few rows: latency; long rows: registers).
-bool four_rows(int T, int threads) { return threads <= 512 && T >= 4 * sms(); }
-
-int fwd_blocks(int T, int rows, int threads) {
-  const long long want = (static_cast<long long>(T) + rows - 1) / rows;
-  const long long cap = static_cast<long long>(sms()) * (1536 / threads > 0 ? 1536 / threads : 1);
-  return static_cast<int>(want < cap ? want : cap);
+// Rows of a block's pass: 4 for blocks of up to 256 threads, 2 up to 512 (registers),
+// 1 for wider rows and where there are too few rows to give every SM a pass.
+int rows_per_pass(int T, int threads) {
+  const int r = threads <= 256 ? 4 : threads <= 512 ? 2 : 1;
+  return T >= r * sms() ? r : 1;
 }
 
-// Blocks of the backward pass (each writes one partial row of the weight
-// gradients). Also the size of the workspace, so a function of T and C alone.
-int bwd_blocks(int T, int rows, int threads) {
-  const long long want = (static_cast<long long>(T) + rows - 1) / rows;
-  const long long cap = static_cast<long long>(sms()) * (768 / threads > 0 ? 768 / threads : 1);
-  return static_cast<int>(want < cap ? want : cap);
+// Blocks of a kernel that fit the GPU at once, at most one per pass. Per SM they are
+// limited by registers; `cache` keeps the occupancy query's answer by warps per block.
+template <typename K>
+int resident_blocks(K kern, int threads, long long passes, int most_per_sm, signed char (&cache)[33]) {
+  const int w = threads / 32;
+  if (!cache[w]) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n < 1) n = 1;
+    cache[w] = static_cast<signed char>(n);
+  }
+  const long long n = static_cast<long long>(sms()) * (cache[w] < most_per_sm ? cache[w] : most_per_sm);
+  return static_cast<int>(passes < n ? passes : n);
 }
-constexpr int kMaxBlocksPerSm = 24;  // 768 / 32
+
+// Partial rows of the weight gradients: at most this many blocks to an SM in the
+// backward pass (each SM's loads stay in flight with fewer).
+constexpr int kMaxBwdBlocksPerSm = 8;
+
+template <typename T, int VEC, int NV, int R>
+int launch_fwd(const NormParams& p, int threads, cudaStream_t st) {
+  static signed char cache[33] = {0};
+  auto kern = layer_norm_fwd_kernel<T, VEC, NV, R>;
+  const int n = resident_blocks(kern, threads, (static_cast<long long>(p.T) + R - 1) / R, 32, cache);
+  kern<<<n, threads, 0, st>>>(p);
+  return launched();
+}
+
+template <typename T, int VEC, int NV, int R, bool PACKED>
+int launch_bwd(const NormParams& p, int threads, int* groups, cudaStream_t st) {
+  static signed char cache[33] = {0};
+  auto kern = layer_norm_bwd_kernel<T, VEC, NV, R, PACKED>;
+  *groups = resident_blocks(kern, threads, (static_cast<long long>(p.T) + R - 1) / R, kMaxBwdBlocksPerSm, cache);
+  kern<<<*groups, threads, 0, st>>>(p);
+  return launched();
+}
 
 template <typename T>
-int norm_fwd(const NormParams& p, cudaStream_t st) {
+int norm_fwd(NormParams p, cudaStream_t st) {
   if (p.C > kMaxCols) {
-    const int n = fwd_blocks(p.T, 1, 1024);
+    const int n = p.T < 2 * sms() ? p.T : 2 * sms();
     layer_norm_fwd_wide_kernel<T><<<n, 1024, 0, st>>>(p);
     return launched();
   }
   RowVec rv(p.C, sizeof(T));
   rv.row(p.x, p.x_stride).row(p.out, p.out_stride);
+  p.w_vec = aligned_to(p.w, 16) && aligned_to(p.b, 16);
   return with_shape(rv.v, p.C, [&](auto vec, auto nv, int threads) {
     constexpr int V = decltype(vec)::value, N = decltype(nv)::value;
-    if (four_rows(p.T, threads))
-      layer_norm_fwd_kernel<T, V, N, 4><<<fwd_blocks(p.T, 4, threads), threads, 0, st>>>(p);
-    else
-      layer_norm_fwd_kernel<T, V, N, 1><<<fwd_blocks(p.T, 1, threads), threads, 0, st>>>(p);
-    return launched();
+    switch (rows_per_pass(p.T, threads)) {
+      case 4: return launch_fwd<T, V, N, 4>(p, threads, st);
+      case 2: return launch_fwd<T, V, N, 2>(p, threads, st);
+      default: return launch_fwd<T, V, N, 1>(p, threads, st);
+    }
   });
 }
 
 template <typename T, bool PACKED>
 int norm_bwd(NormParams p, int* groups, cudaStream_t st) {
   if (p.C > kMaxCols) {
-    const int n = fwd_blocks(p.T, 1, 1024);
+    const int n = p.T < 2 * sms() ? p.T : 2 * sms();
     layer_norm_bwd_wide_kernel<T, PACKED><<<n, 1024, 0, st>>>(p);
     if (p.partial) {
       *groups = p.T < sms() ? p.T : sms();
@@ -545,16 +614,14 @@ int norm_bwd(NormParams p, int* groups, cudaStream_t st) {
   }
   RowVec rv(p.C, sizeof(T));
   rv.row(p.x, p.x_stride).row(p.dy, p.dy_stride).row(p.out, p.out_stride);
+  p.w_vec = aligned_to(p.w, 16);
   return with_shape(rv.v, p.C, [&](auto vec, auto nv, int threads) {
     constexpr int V = decltype(vec)::value, N = decltype(nv)::value;
-    if (four_rows(p.T, threads)) {
-      *groups = bwd_blocks(p.T, 4, threads);
-      layer_norm_bwd_kernel<T, V, N, 4, PACKED><<<*groups, threads, 0, st>>>(p);
-    } else {
-      *groups = bwd_blocks(p.T, 1, threads);
-      layer_norm_bwd_kernel<T, V, N, 1, PACKED><<<*groups, threads, 0, st>>>(p);
+    switch (rows_per_pass(p.T, threads)) {
+      case 4: return launch_bwd<T, V, N, 4, PACKED>(p, threads, groups, st);
+      case 2: return launch_bwd<T, V, N, 2, PACKED>(p, threads, groups, st);
+      default: return launch_bwd<T, V, N, 1, PACKED>(p, threads, groups, st);
     }
-    return launched();
   });
 }
 
@@ -617,7 +684,16 @@ int column_finish(const float* partial, int groups, int arrays, int C, void* out
   f.out[0] = out0;
   f.out[1] = out1;
   f.dtype = dtype;
-  column_finish_kernel<<<dim3((C + 31) / 32, arrays), dim3(32, 16), 0, st>>>(f);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((C + 31) / 32, arrays);
+  lc.blockDim = dim3(32, 32);
+  lc.stream = st;
+  lc.attrs = &attr;
+  lc.numAttrs = 1;
+  if (cudaLaunchKernelEx(&lc, column_finish_kernel, f) != cudaSuccess) return FRATTN_E_CUDA;
   return launched();
 }
 
@@ -678,7 +754,7 @@ int frattn_workspace_bytes_layer_norm_bwd(int T, int C, size_t* bytes) {
   if (!bytes) return FRATTN_E_NULL;
   if (T < 0 || C <= 0) return FRATTN_E_SHAPE;
   // one partial row of the two weight gradients per block
-  const long long blocks = static_cast<long long>(sms()) * (C <= 1024 ? kMaxBlocksPerSm : 8);
+  const long long blocks = static_cast<long long>(sms()) * kMaxBwdBlocksPerSm;
   *bytes = static_cast<size_t>(T < blocks ? (T > 0 ? T : 1) : blocks) * 2 * C * sizeof(float);
   return 0;
 }
