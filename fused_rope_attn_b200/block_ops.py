@@ -19,13 +19,13 @@ buffers are read in place).
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from .fused_attn import _DT, _aligned, _status_word
+from .fused_attn import _DT, _status_word
 
 __all__ = [
     "ACTIVATIONS",
@@ -46,25 +46,30 @@ PACK_BLOCK = 32
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
-class _on:
-    """``torch.cuda.device(dev)`` that costs nothing when dev is already current."""
-
-    __slots__ = ("ctx",)
-
-    def __init__(self, device):
-        self.ctx = None if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _call(name: str, device: torch.device, *args) -> None:
+    """Calls a C entry on ``device`` with its current stream as the last argument."""
+    fn = getattr(_lib.load(), name)
+    i = device.index
+    if i is None or i == torch.cuda.current_device():
+        # the handle alone: torch.cuda.current_stream builds an object around it, 2 us of a
+        # small call's 10
+        stream = _raw_stream(i) if _raw_stream and i is not None else torch.cuda.current_stream(device).cuda_stream
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        _lib.check(rc, name)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(query, device, *sizes) -> int:
+    """Workspace sizes are a function of the shape and the device."""
+    with torch.cuda.device(device):
+        return query(*sizes)
 
 
 def _ptr(t):
@@ -76,7 +81,7 @@ def _workspace(nbytes: int, device) -> torch.Tensor:
 
 
 def _check_rows(name, t, dtypes):
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be on CUDA, got device={t.device}")
     if t.ndim != 2:
         raise ValueError(f"{name} must be 2D [T, C], got {tuple(t.shape)}")
@@ -172,10 +177,8 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
     _check_rows("x", x, tuple(_DT))
     x = _rows(x)
     p = _empty_packed(x.shape[0], x.shape[1], x.dtype, x.device)
-    with _on(x.device):
-        rc = _lib.load().frattn_act_pack(x.data_ptr(), _stride(x), x.shape[0], x.shape[1], _DT[x.dtype],
-                                         p.codes.data_ptr(), p.scales.data_ptr(), _stream(x.device))
-    _lib.check(rc, "frattn_act_pack")
+    _call("frattn_act_pack", x.device, x.data_ptr(), _stride(x), x.shape[0], x.shape[1], _DT[x.dtype],
+          p.codes.data_ptr(), p.scales.data_ptr())
     return p
 
 
@@ -188,10 +191,8 @@ def unpack_activation(p: PackedActivation, *, out: torch.Tensor | None = None) -
         out = torch.empty(p.shape, dtype=p.dtype, device=p.device)
     else:
         out = _check_out_rows(out, p.shape, torch.empty(0, dtype=p.dtype, device=p.device))
-    with _on(p.device):
-        rc = _lib.load().frattn_act_unpack(p.codes.data_ptr(), p.scales.data_ptr(), p.shape[0], p.width,
-                                           _DT[p.dtype], out.data_ptr(), _stride(out), _stream(p.device))
-    _lib.check(rc, "frattn_act_unpack")
+    _call("frattn_act_unpack", p.device, p.codes.data_ptr(), p.scales.data_ptr(), p.shape[0], p.width,
+          _DT[p.dtype], out.data_ptr(), _stride(out))
     return out
 
 
@@ -232,14 +233,13 @@ def layer_norm(
     pd = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
     x = _rows(x)
     out = _check_out_rows(out, (T, C), x)
+    dev = x.device
     mean = rstd = None
     if return_stats:
-        mean, rstd = torch.empty(2, T, dtype=torch.float32, device=x.device).unbind(0)
-    with _on(x.device):
-        rc = _lib.load().frattn_layer_norm(x.data_ptr(), _stride(x), _ptr(weight), _ptr(bias), _DT[pd], T, C,
-                                           float(eps), _DT[x.dtype], out.data_ptr(), _stride(out), _ptr(mean),
-                                           _ptr(rstd), _stream(x.device))
-    _lib.check(rc, "frattn_layer_norm")
+        mean = torch.empty(T, dtype=torch.float32, device=dev)
+        rstd = torch.empty(T, dtype=torch.float32, device=dev)
+    _call("frattn_layer_norm", dev, x.data_ptr(), _stride(x), _ptr(weight), _ptr(bias), _DT[pd], T, C, eps,
+          _DT[x.dtype], out.data_ptr(), _stride(out), _ptr(mean), _ptr(rstd))
     return (out, mean, rstd) if return_stats else out
 
 
@@ -284,17 +284,14 @@ def layer_norm_backward(
     dw = db = ws = None
     nbytes = 0
     if need_param_grads:
-        dw, db = torch.empty(2, C, dtype=pd, device=dev).unbind(0)
-        with _on(dev):
-            nbytes = _lib.workspace_bytes_layer_norm_bwd(T, C)
+        dw = torch.empty(C, dtype=pd, device=dev)
+        db = torch.empty(C, dtype=pd, device=dev)
+        nbytes = _workspace_bytes(_lib.workspace_bytes_layer_norm_bwd, dev, T, C)
         ws = _workspace(nbytes, dev)
-    with _on(dev):
-        rc = _lib.load().frattn_layer_norm_bwd(
-            dout.data_ptr(), _stride(dout), None if packed else x.data_ptr(), 0 if packed else _stride(x),
-            x.codes.data_ptr() if packed else None, x.scales.data_ptr() if packed else None, _ptr(weight), _DT[pd],
-            mean.data_ptr(), rstd.data_ptr(), T, C, _DT[dout.dtype], dx.data_ptr(), C, _ptr(dw), _ptr(db), _ptr(ws),
-            nbytes, _stream(dev))
-    _lib.check(rc, "frattn_layer_norm_bwd")
+    _call("frattn_layer_norm_bwd", dev, dout.data_ptr(), _stride(dout), None if packed else x.data_ptr(),
+          0 if packed else _stride(x), x.codes.data_ptr() if packed else None,
+          x.scales.data_ptr() if packed else None, _ptr(weight), _DT[pd], mean.data_ptr(), rstd.data_ptr(), T, C,
+          _DT[dout.dtype], dx.data_ptr(), C, _ptr(dw), _ptr(db), _ptr(ws), nbytes)
     return dx, dw, db
 
 
@@ -393,16 +390,12 @@ def linear_act(
         p = _empty_packed(T, N, dt, dev)
     if T > 0:
         x, weight = _rows16(x), _rows16(weight)
-        with _on(dev):
-            nbytes = _lib.workspace_bytes_linear_act(T, K, N)
-            ws = _workspace(nbytes, dev) if nbytes else None
-            rc = _lib.load().frattn_linear_act(
-                x.data_ptr(), _row16_stride(x), weight.data_ptr(), _row16_stride(weight), _ptr(bias), _ptr(residual),
-                0 if residual is None else _stride(residual), act, T, K, N, _DT[dt], out.data_ptr(), _stride(out),
-                _ptr(z), N, p.codes.data_ptr() if p is not None else None,
-                p.scales.data_ptr() if p is not None else None, _ptr(ws), nbytes, _status_word(dev).data_ptr(),
-                _stream(dev))
-        _lib.check(rc, "frattn_linear_act")
+        nbytes = _workspace_bytes(_lib.workspace_bytes_linear_act, dev, T, K, N)
+        ws = _workspace(nbytes, dev) if nbytes else None
+        _call("frattn_linear_act", dev, x.data_ptr(), _row16_stride(x), weight.data_ptr(), _row16_stride(weight),
+              _ptr(bias), _ptr(residual), 0 if residual is None else _stride(residual), act, T, K, N, _DT[dt],
+              out.data_ptr(), _stride(out), _ptr(z), N, p.codes.data_ptr() if p is not None else None,
+              p.scales.data_ptr() if p is not None else None, _ptr(ws), nbytes, _status_word(dev).data_ptr())
     if save_preact in (None, "none"):
         return out
     return out, (z if p is None else p)
@@ -472,17 +465,14 @@ def linear_act_backward(
         x = _rows16(x)
     if need_x:
         weight = _rows16(weight)
-    with _on(dev):
-        nbytes = _lib.workspace_bytes_linear_act_bwd(T, K, N)
-        ws = _workspace(nbytes, dev)
-        rc = _lib.load().frattn_linear_act_bwd(
-            dout.data_ptr(), _stride(dout), None if xp else x.data_ptr(), 0 if xp else _row16_stride(x),
-            x.codes.data_ptr() if xp else None, x.scales.data_ptr() if xp else None, weight.data_ptr(),
-            _row16_stride(weight), None if preact is None or zp else preact.data_ptr(),
-            0 if preact is None or zp else _stride(preact), preact.codes.data_ptr() if zp else None,
-            preact.scales.data_ptr() if zp else None, act, T, K, N, _DT[dt], _ptr(dx), K, _ptr(dw), _ptr(db),
-            ws.data_ptr(), nbytes, _status_word(dev).data_ptr(), _stream(dev))
-    _lib.check(rc, "frattn_linear_act_bwd")
+    nbytes = _workspace_bytes(_lib.workspace_bytes_linear_act_bwd, dev, T, K, N)
+    ws = _workspace(nbytes, dev)
+    _call("frattn_linear_act_bwd", dev, dout.data_ptr(), _stride(dout), None if xp else x.data_ptr(),
+          0 if xp else _row16_stride(x), x.codes.data_ptr() if xp else None, x.scales.data_ptr() if xp else None,
+          weight.data_ptr(), _row16_stride(weight), None if preact is None or zp else preact.data_ptr(),
+          0 if preact is None or zp else _stride(preact), preact.codes.data_ptr() if zp else None,
+          preact.scales.data_ptr() if zp else None, act, T, K, N, _DT[dt], _ptr(dx), K, _ptr(dw), _ptr(db),
+          ws.data_ptr(), nbytes, _status_word(dev).data_ptr())
     return dx, dw, db
 
 

@@ -621,6 +621,13 @@ struct GemmPlan {
   size_t partial_bytes;
 };
 
+// The shortest of four estimates, in microseconds of a 64-wide step: whole tiles, dealt
+// out in rounds of all pairs, and the same steps dealt out evenly (Segments), for tiles
+// 256 and 128 wide. With every pair at work a step is bound by what the SMs draw from
+// L2: 0.37 us for 256 x 256 (64 KB) but 0.31 for 256 x 128 (48 KB), measured at
+// 9216 x 3424 -> 1280 (71 us with 256-wide tiles in three rounds, 90 us with 128-wide
+// ones in five); narrow tiles pay only where there are too few wide ones. Even dealing
+// pays for writing and reading the parts (4 TB/s together) and a second kernel.
 GemmPlan gemm_plan(int M, int N, int nk) {
   GemmPlan best{};
   const int P = sm_pairs();
@@ -628,10 +635,10 @@ GemmPlan gemm_plan(int M, int N, int nk) {
   for (int bn : {256, 128}) {
     const long long tiles = static_cast<long long>((M + 255) / 256) * ((N + bn - 1) / bn);
     if (tiles > (1 << 30) / (nk + 1)) continue;
-    const double step_us = bn == 256 ? 0.36 : 0.21;  // one 64-wide step of a 256 x bn tile
+    const double step_us = bn == 256 ? 0.37 : 0.31;
     {
-      const long long waves = (tiles + P - 1) / P;
-      const double us = static_cast<double>(waves) * nk * step_us + 2.0;
+      const long long rounds = (tiles + P - 1) / P;
+      const double us = static_cast<double>(rounds) * nk * step_us;
       if (us < best_us) {
         best_us = us;
         best = GemmPlan{bn, static_cast<int>(tiles), 0, static_cast<int>(tiles < P ? tiles : P), 0};
@@ -643,7 +650,7 @@ GemmPlan gemm_plan(int M, int N, int nk) {
     if (tiles % P != 0) {
       const int pairs = static_cast<int>((total + split - 1) / split);
       const double rows = M < 256 ? M : 256;
-      const double us = split * step_us + 6.0 + 2.0 * pairs * rows * bn * 4 * 2 / 4e6;
+      const double us = split * step_us + 4.0 + 2.0 * pairs * rows * bn * 4 * 2 / 4e6;
       if (us < best_us) {
         best_us = us;
         best = GemmPlan{bn, static_cast<int>(tiles), split, pairs, static_cast<size_t>(2) * pairs * 256 * bn * 4};

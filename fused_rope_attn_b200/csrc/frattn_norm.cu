@@ -9,13 +9,18 @@
 // All sums are kept in 32 bits; the variance is the sum of squared differences
 // from the mean over values held in registers (no difference of large sums).
 //
-// Both are bound by the bytes of the rows. A block holds R whole rows in registers
-// (one vector of up to 8 columns per thread for rows of up to 8192 columns), so every
-// row is read once; the next R rows' loads are issued before the current ones are
-// worked on, and R rows share each block-wide reduction's barrier. The weight
-// gradients stay in the registers of the thread that owns the column over all
-// rows of a block; each block writes one partial row, and column_finish adds
-// the partial rows in a fixed order (no atomics: the same bits every run).
+// Both are bound by the bytes of the rows. A team of 1 to 8 warps works on a row at a
+// time, up to 40 columns to a lane held in registers, so that a row is read from memory
+// once (fewer columns and more warps cost more instructions per value than the memory
+// leaves time for: 8 columns to a lane took 17 us where this takes 10 at 9216 x 1280).
+// The forward takes one row per team and leaves it to the scheduler to overlap them.
+// The backward is persistent, because the weight gradients stay in the registers of
+// the lane that owns the column: its rows come through a ring in shared memory of the
+// team's own, filled by asynchronous 16-byte copies, which hold no registers and,
+// being cut at 16-byte boundaries of the address and not of the row, take rows of any
+// alignment. At the end the teams of a block add their gradients through shared
+// memory, each block writes one partial row, and column_finish adds the partial
+// rows, all in a fixed order (no atomics: the same bits every run).
 #include "frattn_block.cuh"
 
 namespace frattn {
@@ -28,7 +33,7 @@ struct NormParams {
   const void* w;        // [C] or null (ones)
   const void* b;        // [C] or null (zeros), forward only
   int w_f32;            // w, b, dw, db are fp32 (else the element type)
-  int w_vec;            // w and b are 16-byte aligned
+  int w_vec;            // w and b are 16-byte aligned (forward)
   const void* dy;       // [T, C] rows of dy_stride elements, backward only
   long long dy_stride;
   void* out;            // y or dx
@@ -42,35 +47,20 @@ struct NormParams {
 
 namespace {
 
-// Sums over the block's threads of R values (a power of two); every thread gets them.
-// Within a warp the lanes split the values among them as they halve: R - 1 + 5 - log2 R
-// shuffles instead of 5 R. `red` holds 32 R floats and must not be reused before the
-// next barrier but one.
+// Sum over the block's threads (wide rows); every thread gets it. `red` must not be
+// reused before the next barrier but one.
 template <int R>
 __device__ __forceinline__ void block_sum(float (&s)[R], float* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  float t[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) t[r] = s[r];
-  int o = 16;
+  for (int r = 0; r < R; ++r) {
 #pragma unroll
-  for (int n = R; n > 1; n >>= 1, o >>= 1) {
-    const bool up = lane & o;  // this lane keeps the upper half of the values
-#pragma unroll
-    for (int r = 0; r < n / 2; ++r) {
-      const float give = up ? t[r] : t[r + n / 2], keep = up ? t[r + n / 2] : t[r];
-      t[r] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-    }
+    for (int o = 16; o > 0; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
   }
+  const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-  for (int q = 16 / R; q > 0; q >>= 1) t[0] += __shfl_xor_sync(0xffffffffu, t[0], q);
-  // value r now lies in the lanes whose bits 4 .. 5 - log2 R spell r (highest bit first)
-  if (nw == 1) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) s[r] = __shfl_sync(0xffffffffu, t[0], r * (32 / R));
-    return;
+    for (int r = 0; r < R; ++r) red[warp * R + r] = s[r];
   }
-  if (lane % (32 / R) == 0) red[warp * R + lane / (32 / R)] = t[0];
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r) s[r] = 0.f;
@@ -80,108 +70,387 @@ __device__ __forceinline__ void block_sum(float (&s)[R], float* red) {
   }
 }
 
-// Parameter vector (weight or bias) of columns [c, c + VEC) in 32 bits.
-template <typename T, int VEC>
-__device__ __forceinline__ void load_param(const void* p, int f32, int vec, int c, float fill, float (&v)[VEC]) {
-  if (!p) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = fill;
-  } else if (vec) {
-    if (f32) {
-      Vec<float, VEC> x;
-      x.load(static_cast<const float*>(p) + c);
-      x.get(v);
-    } else {
-      Vec<T, VEC> x;
-      x.load(static_cast<const T*>(p) + c);
-      x.get(v);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      v[e] = f32 ? __ldg(static_cast<const float*>(p) + c + e) : elem_f32<T>(static_cast<const T*>(p)[c + e]);
+__device__ __forceinline__ float param_at(const void* p, int f32, int dtype_bf16, int c, float fill) {
+  if (!p) return fill;
+  if (f32) return __ldg(static_cast<const float*>(p) + c);
+  return dtype_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[c]) : __half2float(static_cast<const __half*>(p)[c]);
+}
+
+// ---------------------------------------------------------------- row ring
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, uint32_t bytes) {
+  // reads `bytes` (<= 16) of the 16, the rest of dst is zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Bytes of ring for a row of up to `bytes` bytes at any alignment: the 16-byte pieces of
+// memory that it touches (the row starts address mod 16 bytes into them) and a piece of
+// zeros. Slots are zero from the row's end on to start with and every copy ends in a
+// piece of zeros, so what lies between a row and the last column its team covers is zero
+// always.
+__host__ __device__ inline int row_slot(int bytes) { return (bytes + 15) / 16 * 16 + 32; }
+
+__device__ __forceinline__ uint32_t lead(const uint8_t* row) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u;
+}
+
+// A team's threads (t of n) copy the row at `row` into the slot dst; nothing before
+// `base`, the matrix's first row, is read, nor past the row's end.
+__device__ __forceinline__ void fetch_row(const uint8_t* row, int bytes, const uint8_t* base, uint8_t* dst, int t, int n) {
+  const int off = static_cast<int>(lead(row)), end = off + bytes;
+  const uint8_t* src = row - off;
+  if (t == 0 && src < base) {
+    for (int i = off; i < 16 && i < end; ++i) dst[i] = src[i];
+    t += n;
+  }
+  uint32_t d = smem_u32(dst) + 16 * t;
+  for (int at = 16 * t; at < end + 16; at += 16 * n, d += 16 * n) {
+    const int left = end - at;
+    copy16_async(d, left > 0 ? src + at : row, left < 16 ? (left > 0 ? left : 0) : 16);
   }
 }
 
-template <typename T, int VEC, int NV, int R>
-__global__ void __launch_bounds__(R == 1 ? 1024 : R == 2 ? 512 : 256) layer_norm_fwd_kernel(const NormParams p) {
-  __shared__ __align__(16) float red[2][R * 32];
-  const int nvec = p.C / VEC;
-  float w[NV][VEC], b[NV][VEC];
-  bool has[NV];
+// The team: `warps` warps of the block with a named barrier of their own.
+struct Team {
+  int id, t, n;  // team of the block, thread of the team, threads of a team
+  __device__ __forceinline__ explicit Team(int warps) {
+    n = 32 * warps;
+    id = threadIdx.x / n;
+    t = threadIdx.x - id * n;
+  }
+  __device__ __forceinline__ void sync() const {
+    if (n == 32) __syncwarp();
+    else named_bar_sync(1 + id, n);
+  }
+  // Sums of R values over the team. `red` (8 R floats of the team's) is free again after
+  // the team's next sync.
+  template <int R>
+  __device__ __forceinline__ void sum(float (&s)[R], float* red) const {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
-    has[i] = v < nvec;
-    if (has[i]) {
-      load_param<T, VEC>(p.w, p.w_f32, p.w_vec, v * VEC, 1.f, w[i]);
-      load_param<T, VEC>(p.b, p.w_f32, p.w_vec, v * VEC, 0.f, b[i]);
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
+    if (n == 32) return;
+    if ((t & 31) == 0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) red[(t >> 5) * R + r] = s[r];
+    }
+    sync();
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] = 0.f;
+    for (int w = 0; w < n / 32; ++w) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r] += red[w * R + r];
     }
   }
-  const float inv_c = 1.f / static_cast<float>(p.C);
-  const long long step = static_cast<long long>(gridDim.x) * R;
-  Vec<T, VEC> next[R][NV];
-  auto fetch = [&](long long row0) {
+};
+
+// Zeros in a row's slot from the row's end on.
+__device__ __forceinline__ void clear_tail(uint8_t* slot, int bytes, int slot_bytes, const Team& team) {
+  for (int at = bytes / 16 * 16 + 16 * team.t; at < slot_bytes; at += 16 * team.n)
+    *reinterpret_cast<uint4*>(slot + at) = make_uint4(0, 0, 0, 0);
+}
+
+// A lane's columns: 8 NU of them in units of 8, each unit 8 / VEC vectors of VEC. A warp's
+// columns are consecutive, 256 to a unit; vectors lie 32 VEC columns apart, which makes
+// their addresses one register and constants.
+template <int VEC, int NU>
+__device__ __forceinline__ int lane_col(const Team& team) {
+  return (team.t >> 5) * (NU * 256) + (team.t & 31) * VEC;
+}
+template <int VEC>
+__device__ __forceinline__ int unit_col(int c0, int u, int j) {  // first column of vector j of unit u
+  return c0 + (u * (8 / VEC) + j) * 32 * VEC;
+}
+
+// Units of a warp whose 256 columns all exist (they need no comparisons).
+template <int NU>
+__device__ __forceinline__ int full_units(const Team& team, int C) {
+  const int n = (C - (team.t >> 5) * (NU * 256)) / 256;
+  return n < 0 ? 0 : n;
+}
+
+// Eight values of unit u: f(c, v) loads the vector at column c into v.
+template <int VEC, typename F>
+__device__ __forceinline__ void unit_load(int c0, int u, float (&v)[8], F&& f) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const T* row = static_cast<const T*>(p.x) + (row0 + r) * p.x_stride;
+  for (int j = 0; j < 8 / VEC; ++j) {
+    float x[VEC];
+    f(unit_col<VEC>(c0, u, j), x);
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (has[i] && row0 + r < p.T) next[r][i].load(row + static_cast<size_t>(threadIdx.x + i * blockDim.x) * VEC);
+    for (int e = 0; e < VEC; ++e) v[j * VEC + e] = x[e];
+  }
+}
+// From a row in shared memory.
+template <typename T, int VEC>
+__device__ __forceinline__ void unit_get(const uint8_t* row, int c0, int u, float (&v)[8]) {
+  unit_load<VEC>(c0, u, v, [&](int c, float (&x)[VEC]) {
+    Vec<T, VEC> r;
+#pragma unroll
+    for (int i = 0; i < Vec<T, VEC>::kParts; ++i)
+      raw_words(reinterpret_cast<const typename Vec<T, VEC>::Raw*>(row + c * sizeof(T))[i], r.w + i * Vec<T, VEC>::kPartWords);
+    r.get(x);
+  });
+}
+// From a checkpoint's row in shared memory: codes and scale bytes.
+template <int VEC>
+__device__ __forceinline__ void unit_get_packed(const uint8_t* codes, const uint8_t* scales, int c0, int u, float (&v)[8]) {
+  unit_load<VEC>(c0, u, v, [&](int c, float (&x)[VEC]) {
+    CodeVec<VEC> q;
+    raw_words(*reinterpret_cast<const typename RawVec<VEC>::type*>(codes + c), q.w);
+    q.get(pack_step(scales[c / kPackBlock]), x);
+  });
+}
+// Eight values of unit u to a row of T in global memory.
+template <typename T, int VEC>
+__device__ __forceinline__ void unit_put(T* row, int c0, int u, int full, int C, const float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8 / VEC; ++j) {
+    const int c = unit_col<VEC>(c0, u, j);
+    float f[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = v[j * VEC + e];
+    if (u < full || c < C) Vec<T, VEC>::put(row + c, f);
+  }
+}
+
+// Weights in shared memory in 32 bits, C rounded up to 8 of them (zeros there). For
+// vectors of 8 the two float4 of a vector lie half the array apart, so that the lanes'
+// reads have no bank conflicts.
+template <int VEC>
+__device__ __forceinline__ int param_slot(int c, int C8) {
+  return VEC == 8 ? ((c >> 2) & 1) * (C8 / 2) + (c >> 3) * 4 + (c & 3) : c;
+}
+template <int VEC>
+__device__ __forceinline__ void unit_param(const float* w, int c0, int u, int C8, float (&v)[8]) {
+  unit_load<VEC>(c0, u, v, [&](int c, float (&x)[VEC]) {
+    if constexpr (VEC == 1) {
+      x[0] = w[c];
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(w + (VEC == 8 ? c / 2 : c));
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+      if constexpr (VEC == 8) {
+        const float4 b = *reinterpret_cast<const float4*>(w + C8 / 2 + c / 2);
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+      }
     }
+  });
+}
+
+// The block copies a parameter vector there: eight values to a thread and step, whose
+// loads are in flight together (a block may be a single warp).
+template <typename T, int VEC>
+__device__ __forceinline__ void stage_param(float* to, const void* src, int f32, float fill, int C, int C8) {
+  const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
+#pragma unroll 4
+  for (int c = 8 * static_cast<int>(threadIdx.x); c < C8; c += 8 * static_cast<int>(blockDim.x)) {
+    float v[8];
+    if (!src) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fill;
+    } else if (vec && c + 8 <= C) {
+      if (f32) {
+        Vec<float, 8> x;
+        x.load(static_cast<const float*>(src) + c);
+        x.get(v);
+      } else {
+        Vec<T, 8> x;
+        x.load(static_cast<const T*>(src) + c);
+        x.get(v);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int at = c + e < C ? c + e : C - 1;  // (past C: any value, the gradient there is 0)
+        v[e] = f32 ? __ldg(static_cast<const float*>(src) + at) : elem_f32<T>(static_cast<const T*>(src)[at]);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<float4*>(to + param_slot<VEC>(c + 4 * h, C8)) =
+          make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+  }
+}
+
+// How a block's shared memory is laid out: parameters, then per team the ring and the
+// reduction's floats.
+struct NormLayout {
+  int warps;   // of a team
+  int teams;   // of a block
+  int passes;  // rows of the ring: one worked on, the others on their way
+  int slot;    // ring bytes of a row
+  int cols;                // columns that a team covers, C or more: what the rows and parameters are padded to
+  int params, team_bytes;  // bytes
+};
+
+// Parameters of unit u from global memory (every row reads them: they stay in L1).
+template <typename T, int VEC>
+__device__ __forceinline__ void unit_param_global(const void* p, int f32, int vec, float fill, int c0, int u, int C,
+                                                  float (&v)[8]) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fill;
+  } else if (f32) {
+    unit_load<VEC>(c0, u, v, [&](int c, float (&x)[VEC]) {
+      const float* src = static_cast<const float*>(p) + c;
+      Vec<float, VEC> r;  // (past C: whatever is there, for no output)
+      if (vec) {
+        if (c < C) r.load(src);
+        r.get(x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = c < C ? __ldg(src + e) : 0.f;
+      }
+    });
+  } else {
+    unit_load<VEC>(c0, u, v, [&](int c, float (&x)[VEC]) {
+      const T* src = static_cast<const T*>(p) + c;
+      Vec<T, VEC> r;
+      if (vec) {
+        if (c < C) r.load(src);
+        r.get(x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = c < C ? elem_f32<T>(src[e]) : 0.f;
+      }
+    });
+  }
+}
+
+// Few rows: a block per row.
+template <typename T, int VEC, int NU>
+__global__ void __launch_bounds__(256) layer_norm_fwd_few_kernel(const NormParams p) {
+  __shared__ float red[1][2][8];
+  const Team team(blockDim.x / 32);
+  const long long row = blockIdx.x;
+  const int c0 = lane_col<VEC, NU>(team), full = full_units<NU>(team, p.C);
+  const T* src = static_cast<const T*>(p.x) + row * p.x_stride;
+  float x[NU][8], s[1] = {0.f};
+#pragma unroll
+  for (int u = 0; u < NU; ++u)
+    unit_load<VEC>(c0, u, x[u], [&](int c, float (&v)[VEC]) {
+      Vec<T, VEC> r;
+#pragma unroll
+      for (int i = 0; i < Vec<T, VEC>::kParts * Vec<T, VEC>::kPartWords; ++i) r.w[i] = 0;
+      if (c < p.C) r.load(src + c);
+      r.get(v);
+    });
+#pragma unroll
+  for (int u = 0; u < NU; ++u)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[0] += x[u][e];
+  team.sum(s, red[team.id][0]);
+  const float inv_c = 1.f / static_cast<float>(p.C), mean = s[0] * inv_c;
+  s[0] = 0.f;
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[u][e] -= mean;
+    if (u >= full) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (unit_col<VEC>(c0, u, e / VEC) >= p.C) x[u][e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[0] += x[u][e] * x[u][e];
+  }
+  team.sum(s, red[team.id][1]);
+  const float rstd = rsqrtf(s[0] * inv_c + p.eps);
+  if (team.t == 0) {
+    if (p.mean) p.mean[row] = mean;
+    if (p.rstd) p.rstd[row] = rstd;
+  }
+  T* out = static_cast<T*>(p.out) + row * p.out_stride;
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    float g[8], h[8];
+    unit_param_global<T, VEC>(p.w, p.w_f32, p.w_vec, 1.f, c0, u, p.C, g);
+    unit_param_global<T, VEC>(p.b, p.w_f32, p.w_vec, 0.f, c0, u, p.C, h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[u][e] = x[u][e] * rstd * g[e] + h[e];
+    unit_put<T, VEC>(out, c0, u, full, p.C, x[u]);
+  }
+}
+
+// Many rows: persistent teams whose rows come through the ring.
+template <typename T, int VEC, int NU>
+__global__ void __launch_bounds__(256, NU > 3 ? 3 : 4) layer_norm_fwd_kernel(const NormParams p, const NormLayout l) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* w = reinterpret_cast<float*>(smem);
+  float* b = w + l.cols;
+  const Team team(l.warps);
+  const int c0 = lane_col<VEC, NU>(team), full = full_units<NU>(team, p.C);
+  uint8_t* ring = smem + l.params + team.id * l.team_bytes;
+  float* red = reinterpret_cast<float*>(ring + l.team_bytes) - 16;  // the last 64 bytes of the team's part
+  constexpr int kT = static_cast<int>(sizeof(T));
+  const uint8_t* const base = static_cast<const uint8_t*>(p.x);
+  const long long stride = p.x_stride * kT;
+  const int step = gridDim.x * l.teams, bytes = p.C * kT, first = blockIdx.x * l.teams + team.id;
+  long long fetched = first;
+  int into = 0;
+  auto fetch = [&] {
+    if (fetched < p.T) fetch_row(base + fetched * stride, bytes, base, ring + into * l.slot, team.t, team.n);
+    copies_commit();
+    fetched += step;
+    into = into + 1 == l.passes ? 0 : into + 1;
   };
-  long long row0 = static_cast<long long>(blockIdx.x) * R;
-  fetch(row0);
-  for (; row0 < p.T; row0 += step) {
-    float x[R][NV][VEC], s[R], mean[R];
+  for (int k = 0; k < l.passes; ++k) clear_tail(ring + k * l.slot, bytes, l.slot, team);
+  team.sync();
+  for (int k = 0; k < l.passes - 1; ++k) fetch();
+  stage_param<T, VEC>(w, p.w, p.w_f32, 1.f, p.C, l.cols);
+  stage_param<T, VEC>(b, p.b, p.w_f32, 0.f, p.C, l.cols);
+  __syncthreads();
+  const float inv_c = 1.f / static_cast<float>(p.C);
+  int at = 0;
+  for (long long row = first; row < p.T; row += step) {
+    if (l.passes == 2) copies_wait<0>();
+    else copies_wait<1>();
+    team.sync();  // the row is in the ring, and nobody reads the one before it any more
+    fetch();
+    const uint8_t* src = ring + at * l.slot + lead(base + row * stride);
+    float x[NU][8], s[1] = {0.f};
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      s[r] = 0.f;
+    for (int u = 0; u < NU; ++u) {
+      unit_get<T, VEC>(src, c0, u, x[u]);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        next[r][i].get(x[r][i]);
-        if (has[i]) {  // (rows past the last hold what an earlier pass left there, and go nowhere)
+      for (int e = 0; e < 8; ++e) s[0] += x[u][e];
+    }
+    team.sum(s, red);
+    const float mean = s[0] * inv_c;
+    s[0] = 0.f;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) s[r] += x[r][i][e];
-        }
+    for (int u = 0; u < NU; ++u) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[u][e] -= mean;
+      if (u >= full) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (unit_col<VEC>(c0, u, e / VEC) >= p.C) x[u][e] = 0.f;
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[0] += x[u][e] * x[u][e];
     }
-    fetch(row0 + step);
-    block_sum<R>(s, red[0]);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      mean[r] = s[r] * inv_c;
-      s[r] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (has[i]) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            x[r][i][e] -= mean[r];
-            s[r] += x[r][i][e] * x[r][i][e];
-          }
-        }
+    team.sum(s, red + 8);
+    const float rstd = rsqrtf(s[0] * inv_c + p.eps);
+    if (team.t == 0) {
+      if (p.mean) p.mean[row] = mean;
+      if (p.rstd) p.rstd[row] = rstd;
     }
-    block_sum<R>(s, red[1]);
+    T* out = static_cast<T*>(p.out) + row * p.out_stride;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const long long row = row0 + r;
-      if (row >= p.T) break;
-      const float rstd = rsqrtf(s[r] * inv_c + p.eps);
-      if (threadIdx.x == 0) {
-        if (p.mean) p.mean[row] = mean[r];
-        if (p.rstd) p.rstd[row] = rstd;
-      }
-      T* out = static_cast<T*>(p.out) + row * p.out_stride;
+    for (int u = 0; u < NU; ++u) {
+      float g[8], h[8];
+      unit_param<VEC>(w, c0, u, l.cols, g);
+      unit_param<VEC>(b, c0, u, l.cols, h);
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (has[i]) {
-          float y[VEC];
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) y[e] = x[r][i][e] * rstd * w[i][e] + b[i][e];
-          Vec<T, VEC>::put(out + static_cast<size_t>(threadIdx.x + i * blockDim.x) * VEC, y);
-        }
+      for (int e = 0; e < 8; ++e) x[u][e] = x[u][e] * rstd * g[e] + h[e];
+      unit_put<T, VEC>(out, c0, u, full, p.C, x[u]);
     }
+    at = at + 1 == l.passes ? 0 : at + 1;
   }
 }
 
@@ -189,6 +458,7 @@ __global__ void __launch_bounds__(R == 1 ? 1024 : R == 2 ? 512 : 256) layer_norm
 // (from L2 after the first).
 template <typename T>
 __global__ void __launch_bounds__(1024) layer_norm_fwd_wide_kernel(const NormParams p) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   __shared__ float red[2][32];
   const float inv_c = 1.f / static_cast<float>(p.C);
   for (long long row = blockIdx.x; row < p.T; row += gridDim.x) {
@@ -210,137 +480,182 @@ __global__ void __launch_bounds__(1024) layer_norm_fwd_wide_kernel(const NormPar
       if (p.rstd) p.rstd[row] = rstd;
     }
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
-      float w[1], b[1];
-      load_param<T, 1>(p.w, p.w_f32, 0, c, 1.f, w);
-      load_param<T, 1>(p.b, p.w_f32, 0, c, 0.f, b);
-      out[c] = f32_elem<T>((elem_f32<T>(x[c]) - mean) * rstd * w[0] + b[0]);
+      const float w = param_at(p.w, p.w_f32, kBf16, c, 1.f), b = param_at(p.b, p.w_f32, kBf16, c, 0.f);
+      out[c] = f32_elem<T>((elem_f32<T>(x[c]) - mean) * rstd * w + b);
     }
   }
 }
 
-// VEC values of an input row: 16/32-bit elements or checkpoint codes.
-template <typename T, int VEC, bool PACKED>
-struct NormIn {
-  Vec<T, VEC> v;
-  __device__ __forceinline__ void load(const NormParams& p, long long row, int vec) {
-    v.load(static_cast<const T*>(p.x) + row * p.x_stride + static_cast<size_t>(vec) * VEC);
-  }
-  __device__ __forceinline__ void get(float (&f)[VEC]) const { v.get(f); }
-};
-template <typename T, int VEC>
-struct NormIn<T, VEC, true> {
-  CodeVec<VEC> c;
-  uint32_t scale;
-  __device__ __forceinline__ void load(const NormParams& p, long long row, int vec) {
-    const long long nb = pack_blocks(p.C);
-    c.load(p.codes + row * nb * kPackBlock + static_cast<size_t>(vec) * VEC);
-    scale = __ldg(p.scales + row * nb + vec * VEC / kPackBlock);
-  }
-  __device__ __forceinline__ void get(float (&f)[VEC]) const { c.get(pack_step(scale), f); }
-};
-
-template <typename T, int VEC, int NV, int R, bool PACKED>
-__global__ void __launch_bounds__(R == 1 ? 1024 : R == 2 ? 512 : 256) layer_norm_bwd_kernel(const NormParams p) {
-  __shared__ __align__(16) float red[2][2 * R * 32];
-  const int nvec = p.C / VEC;
-  float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
-  bool has[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
-    has[i] = v < nvec;
-    if (has[i]) load_param<T, VEC>(p.w, p.w_f32, p.w_vec, v * VEC, 1.f, w[i]);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) dw[i][e] = db[i][e] = 0.f;
-  }
-  const float inv_c = 1.f / static_cast<float>(p.C);
-  const long long step = static_cast<long long>(gridDim.x) * R;
-  NormIn<T, VEC, PACKED> nx[R][NV];
-  Vec<T, VEC> ny[R][NV];
-  float nmean[R], nrstd[R];
-  auto fetch = [&](long long row0) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const long long row = row0 + r;
-      nmean[r] = nrstd[r] = 0.f;
-      if (row < p.T) {
-        nmean[r] = __ldg(p.mean + row);
-        nrstd[r] = __ldg(p.rstd + row);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int v = threadIdx.x + i * blockDim.x;
-          if (has[i]) {
-            nx[r][i].load(p, row, v);
-            ny[r][i].load(static_cast<const T*>(p.dy) + row * p.dy_stride + static_cast<size_t>(v) * VEC);
-          }
-        }
-      }
+template <typename T, int VEC, int NU, bool PACKED>
+__global__ void __launch_bounds__(384) layer_norm_bwd_kernel(const NormParams p, const NormLayout l) {
+  constexpr bool kHold = NU <= 3;  // g and h of the row stay in registers between its two uses
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* w = reinterpret_cast<float*>(smem);
+  const Team team(l.warps);
+  const int c0 = lane_col<VEC, NU>(team), full = full_units<NU>(team, p.C);
+  uint8_t* ring = smem + l.params + team.id * l.team_bytes;
+  float* red = reinterpret_cast<float*>(ring + l.team_bytes) - 16;  // the last 64 bytes of the team's part
+  constexpr int kT = static_cast<int>(sizeof(T));
+  const int nb = static_cast<int>(pack_blocks(p.C)), bytes = p.C * kT, xbytes = PACKED ? nb * kPackBlock : bytes;
+  const int off_x = row_slot(l.cols * kT), off_s = off_x + row_slot(PACKED ? l.cols : l.cols * kT);
+  const uint8_t* const ybase = static_cast<const uint8_t*>(p.dy);
+  const uint8_t* const xbase = PACKED ? reinterpret_cast<const uint8_t*>(p.codes) : static_cast<const uint8_t*>(p.x);
+  const long long yrow = p.dy_stride * kT, xrow = PACKED ? xbytes : p.x_stride * kT;
+  const int step = gridDim.x * l.teams, first = blockIdx.x * l.teams + team.id;
+  long long fetched = first;
+  int into = 0;
+  auto fetch = [&] {
+    if (fetched < p.T) {
+      uint8_t* dst = ring + into * l.slot;
+      fetch_row(ybase + fetched * yrow, bytes, ybase, dst, team.t, team.n);
+      fetch_row(xbase + fetched * xrow, xbytes, xbase, dst + off_x, team.t, team.n);
+      if constexpr (PACKED) fetch_row(p.scales + fetched * nb, nb, p.scales, dst + off_s, team.t, team.n);
     }
+    copies_commit();
+    fetched += step;
+    into = into + 1 == l.passes ? 0 : into + 1;
   };
-  int phase = 0;
-  long long row0 = static_cast<long long>(blockIdx.x) * R;
-  fetch(row0);
-  for (; row0 < p.T; row0 += step, phase ^= 1) {
-    float h[R][NV][VEC], d[R][NV][VEC], rstd[R], s[2 * R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      s[2 * r] = s[2 * r + 1] = 0.f;
-      rstd[r] = nrstd[r];
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (has[i] && row0 + r < p.T) {
-          nx[r][i].get(h[r][i]);
-          ny[r][i].get(d[r][i]);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float y = d[r][i][e], t = (h[r][i][e] - nmean[r]) * rstd[r], g = y * w[i][e];
-            dw[i][e] += y * t;
-            db[i][e] += y;
-            s[2 * r] += g;
-            s[2 * r + 1] += g * t;
-            h[r][i][e] = t;
-            d[r][i][e] = g;
-          }
-        }
-    }
-    fetch(row0 + step);
-    block_sum<2 * R>(s, red[phase]);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const long long row = row0 + r;
-      if (row >= p.T) break;
-      const float c1 = s[2 * r] * inv_c, c2 = s[2 * r + 1] * inv_c;
-      T* out = static_cast<T*>(p.out) + row * p.out_stride;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (has[i]) {
-          float o[VEC];
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) o[e] = rstd[r] * (d[r][i][e] - c1 - h[r][i][e] * c2);
-          Vec<T, VEC>::put(out + static_cast<size_t>(threadIdx.x + i * blockDim.x) * VEC, o);
-        }
-    }
+  for (int k = 0; k < l.passes; ++k) {
+    uint8_t* slot = ring + k * l.slot;
+    clear_tail(slot, bytes, off_x, team);
+    clear_tail(slot + off_x, xbytes, off_s - off_x, team);
+    if constexpr (PACKED) clear_tail(slot + off_s, nb, l.slot - off_s, team);
   }
-  if (p.partial) {
-    float* mine = p.partial + static_cast<size_t>(blockIdx.x) * 2 * p.C;
+  team.sync();
+  for (int k = 0; k < l.passes - 1; ++k) fetch();
+  stage_param<T, VEC>(w, p.w, p.w_f32, 1.f, p.C, l.cols);
+  __syncthreads();
+  const float inv_c = 1.f / static_cast<float>(p.C);
+  uint64_t dw[NU][4], db[NU][4];  // pairs of neighbouring columns
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (has[i]) {
+  for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          mine[static_cast<size_t>(v) * VEC + e] = dw[i][e];
-          mine[p.C + static_cast<size_t>(v) * VEC + e] = db[i][e];
+    for (int e = 0; e < 4; ++e) dw[u][e] = db[u][e] = 0;
+  float nmean = first < p.T ? __ldg(p.mean + first) : 0.f, nrstd = first < p.T ? __ldg(p.rstd + first) : 0.f;
+  int at = 0;
+  for (long long row = first; row < p.T; row += step) {
+    const float mean = nmean, rstd = nrstd;
+    if (row + step < p.T) {
+      nmean = __ldg(p.mean + row + step);
+      nrstd = __ldg(p.rstd + row + step);
+    }
+    if (l.passes == 2) copies_wait<0>();
+    else copies_wait<1>();
+    team.sync();  // the row is in the ring, and nobody reads the one before it any more
+    fetch();
+    const uint8_t* slot = ring + at * l.slot;
+    const uint8_t* sy = slot + lead(ybase + row * yrow);
+    const uint8_t* sx = slot + off_x + (PACKED ? 0 : lead(xbase + row * xrow));
+    const uint8_t* ss = slot + off_s + (PACKED ? lead(p.scales + row * nb) : 0);
+    const uint64_t nmean2 = both(-mean), rstd2 = both(rstd);
+    // unit u: dy, g = dy w and h = (x - mean) rstd, in pairs (dy and g are zero past column C)
+    auto values = [&](int u, uint64_t (&d)[4], uint64_t (&g)[4], uint64_t (&h)[4]) {
+      float a[8], x[8], ww[8];
+      unit_get<T, VEC>(sy, c0, u, a);
+      if constexpr (PACKED) unit_get_packed<VEC>(sx, ss, c0, u, x);
+      else unit_get<T, VEC>(sx, c0, u, x);
+      unit_param<VEC>(w, c0, u, l.cols, ww);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d[e] = f2pack(a[2 * e], a[2 * e + 1]);
+        g[e] = mul2(d[e], f2pack(ww[2 * e], ww[2 * e + 1]));
+        h[e] = mul2(add2(f2pack(x[2 * e], x[2 * e + 1]), nmean2), rstd2);
+      }
+    };
+    uint64_t s1 = 0, s2 = 0;
+    uint64_t keep_g[kHold ? NU : 1][4], keep_h[kHold ? NU : 1][4];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      if constexpr (!kHold) asm volatile("" ::: "memory");  // one unit's loads at a time: the sums take the registers
+      uint64_t d[4], g[4], h[4];
+      values(u, d, g, h);
+      if constexpr (kHold) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          keep_g[u][e] = g[e];
+          keep_h[u][e] = h[e];
         }
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dw[u][e] = fma2(d[e], h[e], dw[u][e]);
+        db[u][e] = add2(db[u][e], d[e]);
+        s1 = add2(s1, g[e]);
+        s2 = fma2(g[e], h[e], s2);
+      }
     }
+    float s[2], t0, t1;
+    f2unpack(s1, t0, t1);
+    s[0] = t0 + t1;
+    f2unpack(s2, t0, t1);
+    s[1] = t0 + t1;
+    team.sum(s, red);
+    const uint64_t c1 = both(-s[0] * inv_c), c2 = both(-s[1] * inv_c);
+    T* out = static_cast<T*>(p.out) + row * p.out_stride;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      uint64_t g[4], h[4];
+      if constexpr (kHold) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          g[e] = keep_g[u][e];
+          h[e] = keep_h[u][e];
+        }
+      } else {
+        asm volatile("" ::: "memory");
+        uint64_t d[4];
+        values(u, d, g, h);
+      }
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f2unpack(mul2(fma2(h[e], c2, add2(g[e], c1)), rstd2), o[2 * e], o[2 * e + 1]);
+      unit_put<T, VEC>(out, c0, u, full, p.C, o);
+    }
+    at = at + 1 == l.passes ? 0 : at + 1;
+  }
+  if (!p.partial) return;
+  griddep_launch_dependents();
+  // the block's teams add their columns' sums: each in its own part of shared memory
+  copies_wait<0>();
+  __syncthreads();
+  float* mine = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int u = 0; u < NU; ++u)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = unit_col<VEC>(c0, u, j / VEC) + j % VEC;
+      float a0, a1, b0, b1;
+      f2unpack(dw[u][j / 2], a0, a1);
+      f2unpack(db[u][j / 2], b0, b1);
+      if (c < p.C) {
+        mine[c] = j & 1 ? a1 : a0;
+        mine[p.C + c] = j & 1 ? b1 : b0;
+      }
+    }
+  __syncthreads();
+  float* part = p.partial + static_cast<size_t>(blockIdx.x) * 2 * p.C;
+  for (int c = threadIdx.x; c < 2 * p.C; c += blockDim.x) {
+    float sum = 0.f;
+    for (int q = 0; q < l.teams; ++q) sum += reinterpret_cast<const float*>(smem + l.params + q * l.team_bytes)[c];
+    part[c] = sum;
   }
 }
 
 // More than 8192 columns: dx by one block per row (the row is read twice), the
 // weight gradients by one thread per column over a strip of rows.
 template <typename T, bool PACKED>
+__device__ __forceinline__ float wide_x(const NormParams& p, long long row, int c) {
+  if constexpr (PACKED) {
+    const long long nb = pack_blocks(p.C);
+    return static_cast<float>(__ldg(p.codes + row * nb * kPackBlock + c)) * pack_step(__ldg(p.scales + row * nb + c / kPackBlock));
+  } else {
+    return elem_f32<T>(static_cast<const T*>(p.x)[row * p.x_stride + c]);
+  }
+}
+
+template <typename T, bool PACKED>
 __global__ void __launch_bounds__(1024) layer_norm_bwd_wide_kernel(const NormParams p) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   __shared__ float red[2][64];
   const float inv_c = 1.f / static_cast<float>(p.C);
   int phase = 0;
@@ -350,26 +665,15 @@ __global__ void __launch_bounds__(1024) layer_norm_bwd_wide_kernel(const NormPar
     T* out = static_cast<T*>(p.out) + row * p.out_stride;
     float s[2] = {0.f, 0.f};
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
-      float w[1];
-      load_param<T, 1>(p.w, p.w_f32, 0, c, 1.f, w);
-      NormIn<T, 1, PACKED> in;
-      float x[1];
-      in.load(p, row, c);
-      in.get(x);
-      const float g = elem_f32<T>(dy[c]) * w[0];
+      const float g = elem_f32<T>(dy[c]) * param_at(p.w, p.w_f32, kBf16, c, 1.f);
       s[0] += g;
-      s[1] += g * (x[0] - mean) * rstd;
+      s[1] += g * (wide_x<T, PACKED>(p, row, c) - mean) * rstd;
     }
     block_sum<2>(s, red[phase]);
     const float c1 = s[0] * inv_c, c2 = s[1] * inv_c;
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
-      float w[1];
-      load_param<T, 1>(p.w, p.w_f32, 0, c, 1.f, w);
-      NormIn<T, 1, PACKED> in;
-      float x[1];
-      in.load(p, row, c);
-      in.get(x);
-      out[c] = f32_elem<T>(rstd * (elem_f32<T>(dy[c]) * w[0] - c1 - (x[0] - mean) * rstd * c2));
+      const float g = elem_f32<T>(dy[c]) * param_at(p.w, p.w_f32, kBf16, c, 1.f);
+      out[c] = f32_elem<T>(rstd * (g - c1 - (wide_x<T, PACKED>(p, row, c) - mean) * rstd * c2));
     }
   }
 }
@@ -380,12 +684,8 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_wide_cols_kernel(const Nor
   if (c >= p.C) return;
   float dw = 0.f, db = 0.f;
   for (long long row = blockIdx.y; row < p.T; row += gridDim.y) {
-    NormIn<T, 1, PACKED> in;
-    float x[1];
-    in.load(p, row, c);
-    in.get(x);
     const float d = elem_f32<T>(static_cast<const T*>(p.dy)[row * p.dy_stride + c]);
-    dw += d * (x[0] - __ldg(p.mean + row)) * __ldg(p.rstd + row);
+    dw += d * (wide_x<T, PACKED>(p, row, c) - __ldg(p.mean + row)) * __ldg(p.rstd + row);
     db += d;
   }
   p.partial[static_cast<size_t>(blockIdx.y) * 2 * p.C + c] = dw;
@@ -522,63 +822,92 @@ int sms() {
 
 int launched() { return cudaGetLastError() == cudaSuccess ? 0 : FRATTN_E_CUDA; }
 
-constexpr int kMaxCols = 8192;  // widest row held in registers (1024 threads x 8 columns)
+constexpr int kMaxCols = 8192;  // widest row held in registers (8 warps of 1024 columns)
 
-// Threads for nvec vectors, NV to a thread.
-int threads_for(int nvec, int nv) { return ((nvec + nv - 1) / nv + 31) / 32 * 32; }
+constexpr int kSmemPerSm = 227 * 1024;
 
-// Vectors to a thread: as few as 1024 threads allow, and at least enough that a
-// block of scalar columns stays under 512 threads where it can.
-template <typename F>
-int with_shape(int vec, int C, F&& f) {
-  const int nvec = C / vec;
-  if (vec == 8) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 1>(), threads_for(nvec, 1));
-  if (vec == 4) return f(std::integral_constant<int, 4>(), std::integral_constant<int, 2>(), threads_for(nvec, 2));
-  if (C <= 2048) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 4>(), threads_for(nvec, 4));
-  return f(std::integral_constant<int, 1>(), std::integral_constant<int, 8>(), threads_for(nvec, 8));
-}
-
-// Rows of a block's pass: 4 for blocks of up to 256 threads, 2 up to 512 (registers),
-// 1 for wider rows and where there are too few rows to give every SM a pass.
-int rows_per_pass(int T, int threads) {
-  const int r = threads <= 256 ? 4 : threads <= 512 ? 2 : 1;
-  return T >= r * sms() ? r : 1;
-}
-
-// Blocks of a kernel that fit the GPU at once, at most one per pass. Per SM they are
-// limited by registers; `cache` keeps the occupancy query's answer by warps per block.
-template <typename K>
-int resident_blocks(K kern, int threads, long long passes, int most_per_sm, signed char (&cache)[33]) {
-  const int w = threads / 32;
-  if (!cache[w]) {
-    int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n < 1) n = 1;
-    cache[w] = static_cast<signed char>(n);
+// Calls f<VEC, NU>() for rows of C columns read in vectors of vec by teams of `warps`.
+template <int VEC, typename F>
+int with_units(int units, F&& f) {
+  switch (units) {
+    case 1: return f(std::integral_constant<int, VEC>(), std::integral_constant<int, 1>());
+    case 2: return f(std::integral_constant<int, VEC>(), std::integral_constant<int, 2>());
+    case 3: return f(std::integral_constant<int, VEC>(), std::integral_constant<int, 3>());
+    case 4: return f(std::integral_constant<int, VEC>(), std::integral_constant<int, 4>());
+    default: return f(std::integral_constant<int, VEC>(), std::integral_constant<int, 5>());
   }
-  const long long n = static_cast<long long>(sms()) * (cache[w] < most_per_sm ? cache[w] : most_per_sm);
-  return static_cast<int>(passes < n ? passes : n);
+}
+template <typename F>
+int with_shape(int vec, int C, int warps, F&& f) {
+  const int units = (C + 256 * warps - 1) / (256 * warps);  // of 8 columns to a lane
+  if (vec == 8) return with_units<8>(units, f);
+  if (vec == 4) return with_units<4>(units, f);
+  return with_units<1>(units, f);
+}
+// Warps to a row of the forward: as few as 40 columns to a lane allow (32 where they are
+// single columns, whose addresses take registers too).
+int team_warps(int C, int vec) { return vec == 1 ? (C + 1023) / 1024 : (C + 1279) / 1280; }
+// Of the backward, whose lanes hold two sums a column besides: a warp for up to 1280
+// columns in vectors of 8 (two warps, which have to wait for each other, took 75 us
+// where one takes 57 at 32768 x 1280), else 32 columns to a lane. Twelve warps to an SM:
+// sixteen leave 128 registers to a thread, and spill (73 us there).
+int bwd_team_warps(int C, int vec, bool packed) {
+  if (vec == 8 && !packed && C <= 1280) return 1;
+  const int w = (C + 1023) / 1024;
+  return w < 8 ? w : 8;
+}
+// With this few rows to an SM latency counts: 8 columns to a lane, up to 8 warps.
+constexpr int kFewRows = 2;
+int short_team_warps(int C) {
+  const int w = (C + 255) / 256;
+  return w < 8 ? w : 8;
 }
 
-// Partial rows of the weight gradients: at most this many blocks to an SM in the
-// backward pass (each SM's loads stay in flight with fewer).
-constexpr int kMaxBwdBlocksPerSm = 8;
-
-template <typename T, int VEC, int NV, int R>
-int launch_fwd(const NormParams& p, int threads, cudaStream_t st) {
-  static signed char cache[33] = {0};
-  auto kern = layer_norm_fwd_kernel<T, VEC, NV, R>;
-  const int n = resident_blocks(kern, threads, (static_cast<long long>(p.T) + R - 1) / R, 32, cache);
-  kern<<<n, threads, 0, st>>>(p);
-  return launched();
+// Teams of a block and rows of their rings: as many teams as fit `threads` and the shared
+// memory of 1 / blocks_per_sm of an SM with rings of three rows, unless fewer than half
+// of them do (then two rows); of these no more than the rows, dealt out evenly, keep
+// busy to the end.
+template <typename F>
+NormLayout norm_layout(int T, int C, int warps, int threads, int blocks_per_sm, int params, int least_team_bytes,
+                       F&& slot_of_cols) {
+  NormLayout l;
+  l.warps = warps;
+  l.cols = 256 * warps * ((C + 256 * warps - 1) / (256 * warps));
+  l.params = params * l.cols * 4;
+  l.slot = slot_of_cols(l.cols);
+  const int most = threads / (32 * warps) < 15 || warps == 1 ? threads / (32 * warps) : 15;  // (named barriers 1 to 15)
+  const int room = kSmemPerSm / blocks_per_sm - 1024 - l.params;
+  auto bytes = [&](int passes) {
+    const int b = passes * l.slot > least_team_bytes ? passes * l.slot : least_team_bytes;
+    return (b + 15) / 16 * 16 + 64;  // + the reduction's floats
+  };
+  l.passes = 2 * (room / bytes(3)) >= most ? 3 : 2;
+  l.team_bytes = bytes(l.passes);
+  const int fit = room / l.team_bytes;
+  l.teams = most < fit ? most : fit;
+  if (l.teams < 1) l.teams = 1;
+  const long long blocks = static_cast<long long>(sms()) * blocks_per_sm;
+  const long long rows = (T + blocks * l.teams - 1) / (blocks * l.teams);  // of the busiest team
+  l.teams = static_cast<int>((T + blocks * rows - 1) / (blocks * rows));
+  return l;
 }
 
-template <typename T, int VEC, int NV, int R, bool PACKED>
-int launch_bwd(const NormParams& p, int threads, int* groups, cudaStream_t st) {
-  static signed char cache[33] = {0};
-  auto kern = layer_norm_bwd_kernel<T, VEC, NV, R, PACKED>;
-  *groups = resident_blocks(kern, threads, (static_cast<long long>(p.T) + R - 1) / R, kMaxBwdBlocksPerSm, cache);
-  kern<<<*groups, threads, 0, st>>>(p);
-  return launched();
+// Rings of more than 48 KB are allowed once per kernel and device.
+template <typename K>
+bool allow_ring(K kern, unsigned long long& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerSm) != cudaSuccess) return false;
+  done |= bit;
+  return true;
+}
+
+int norm_blocks(int T, const NormLayout& l, int blocks_per_sm) {
+  const long long want = (static_cast<long long>(T) + l.teams - 1) / l.teams;
+  const long long cap = static_cast<long long>(sms()) * blocks_per_sm;
+  return static_cast<int>(want < cap ? want : cap);
 }
 
 template <typename T>
@@ -590,19 +919,29 @@ int norm_fwd(NormParams p, cudaStream_t st) {
   }
   RowVec rv(p.C, sizeof(T));
   rv.row(p.x, p.x_stride).row(p.out, p.out_stride);
-  p.w_vec = aligned_to(p.w, 16) && aligned_to(p.b, 16);
-  return with_shape(rv.v, p.C, [&](auto vec, auto nv, int threads) {
-    constexpr int V = decltype(vec)::value, N = decltype(nv)::value;
-    switch (rows_per_pass(p.T, threads)) {
-      case 4: return launch_fwd<T, V, N, 4>(p, threads, st);
-      case 2: return launch_fwd<T, V, N, 2>(p, threads, st);
-      default: return launch_fwd<T, V, N, 1>(p, threads, st);
-    }
+  if (p.T <= kFewRows * sms()) {
+    p.w_vec = aligned_to(p.w, 16) && aligned_to(p.b, 16);
+    const int warps = short_team_warps(p.C);
+    return with_shape(rv.v, p.C, warps, [&](auto vec, auto nu) {
+      layer_norm_fwd_few_kernel<T, decltype(vec)::value, decltype(nu)::value><<<p.T, 32 * warps, 0, st>>>(p);
+      return launched();
+    });
+  }
+  const int warps = team_warps(p.C, rv.v);
+  const int blocks = (p.C + 256 * warps - 1) / (256 * warps) > 3 ? 3 : 4;  // of 256 threads to an SM, by registers
+  const NormLayout l = norm_layout(p.T, p.C, warps, 256, blocks, 2, 0,
+                                   [](int cols) { return row_slot(cols * static_cast<int>(sizeof(T))); });
+  return with_shape(rv.v, p.C, warps, [&](auto vec, auto nu) {
+    auto kern = layer_norm_fwd_kernel<T, decltype(vec)::value, decltype(nu)::value>;
+    static unsigned long long ring_ok = 0;
+    if (!allow_ring(kern, ring_ok)) return static_cast<int>(FRATTN_E_CUDA);
+    kern<<<norm_blocks(p.T, l, blocks), 32 * l.warps * l.teams, l.params + l.teams * l.team_bytes, st>>>(p, l);
+    return launched();
   });
 }
 
 template <typename T, bool PACKED>
-int norm_bwd(NormParams p, int* groups, cudaStream_t st) {
+int norm_bwd(const NormParams& p, int* groups, cudaStream_t st) {
   if (p.C > kMaxCols) {
     const int n = p.T < 2 * sms() ? p.T : 2 * sms();
     layer_norm_bwd_wide_kernel<T, PACKED><<<n, 1024, 0, st>>>(p);
@@ -614,14 +953,19 @@ int norm_bwd(NormParams p, int* groups, cudaStream_t st) {
   }
   RowVec rv(p.C, sizeof(T));
   rv.row(p.x, p.x_stride).row(p.dy, p.dy_stride).row(p.out, p.out_stride);
-  p.w_vec = aligned_to(p.w, 16);
-  return with_shape(rv.v, p.C, [&](auto vec, auto nv, int threads) {
-    constexpr int V = decltype(vec)::value, N = decltype(nv)::value;
-    switch (rows_per_pass(p.T, threads)) {
-      case 4: return launch_bwd<T, V, N, 4, PACKED>(p, threads, groups, st);
-      case 2: return launch_bwd<T, V, N, 2, PACKED>(p, threads, groups, st);
-      default: return launch_bwd<T, V, N, 1, PACKED>(p, threads, groups, st);
-    }
+  const int warps = p.T <= kFewRows * sms() ? short_team_warps(p.C) : bwd_team_warps(p.C, rv.v, PACKED);
+  const int gradients = 2 * p.C * 4;  // a team's, in the end
+  const NormLayout l = norm_layout(p.T, p.C, warps, 384, 1, 1, gradients, [](int cols) {
+    const int row = row_slot(cols * static_cast<int>(sizeof(T)));
+    return row + (PACKED ? row_slot(cols) + row_slot(cols / kPackBlock) : row);
+  });
+  return with_shape(rv.v, p.C, l.warps, [&](auto vec, auto nu) {
+    auto kern = layer_norm_bwd_kernel<T, decltype(vec)::value, decltype(nu)::value, PACKED>;
+    static unsigned long long ring_ok = 0;
+    if (!allow_ring(kern, ring_ok)) return static_cast<int>(FRATTN_E_CUDA);
+    *groups = norm_blocks(p.T, l, 1);
+    kern<<<*groups, 32 * l.warps * l.teams, l.params + l.teams * l.team_bytes, st>>>(p, l);
+    return launched();
   });
 }
 
@@ -754,7 +1098,7 @@ int frattn_workspace_bytes_layer_norm_bwd(int T, int C, size_t* bytes) {
   if (!bytes) return FRATTN_E_NULL;
   if (T < 0 || C <= 0) return FRATTN_E_SHAPE;
   // one partial row of the two weight gradients per block
-  const long long blocks = static_cast<long long>(sms()) * kMaxBwdBlocksPerSm;
+  const long long blocks = sms();
   *bytes = static_cast<size_t>(T < blocks ? (T > 0 ? T : 1) : blocks) * 2 * C * sizeof(float);
   return 0;
 }
