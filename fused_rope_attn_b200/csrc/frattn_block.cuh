@@ -303,23 +303,47 @@ __device__ __forceinline__ void act_f2(float& a, float& b) {
   }
 }
 
+// Derivatives of two values at a time, in place.
 template <int ACT>
-__device__ __forceinline__ float act_grad_f(float z) {
-  if constexpr (ACT == FRATTN_ACT_RELU) {
-    return z > 0.f ? 1.f : (z != z ? z : 0.f);
-  } else if constexpr (ACT == FRATTN_ACT_GELU) {
-    float e;
-    const float c = normal_cdf(z, e);
-    return fmaf(z * e, 0.3989422804014327f, c);
+__device__ __forceinline__ void act_grad_f2(float& a, float& b) {
+  if constexpr (ACT == FRATTN_ACT_GELU) {  // normal_cdf's steps, and z e^(-z^2 / 2) / sqrt(2 pi)
+    const uint64_t z = f2pack(a, b);
+    float t0, t1, e0, e1, q0, q1;
+    f2unpack(fma2(f2pack(fabsf(a), fabsf(b)), both(0.23164191f), both(1.f)), t0, t1);
+    const uint64_t t = f2pack(rcp_fast(t0), rcp_fast(t1));
+    f2unpack(mul2(mul2(z, both(-0.7213475204444817f)), z), e0, e1);
+    const uint64_t e = f2pack(exp2_fast(e0), exp2_fast(e1));
+    uint64_t q = fma2(t, both(0.5307027145f), both(-0.7265760135f));
+    q = fma2(q, t, both(0.7107068705f));
+    q = fma2(q, t, both(-0.142248368f));
+    q = fma2(q, t, both(0.127414796f));
+    f2unpack(mul2(mul2(q, t), e), q0, q1);
+    const uint64_t c = f2pack(a < 0.f ? q0 : 1.f - q0, b < 0.f ? q1 : 1.f - q1);
+    f2unpack(fma2(mul2(z, e), both(0.3989422804014327f), c), a, b);
   } else if constexpr (ACT == FRATTN_ACT_GELU_TANH) {
-    const float s = sigmoid_f(1.5957691216057308f * z * (1.f + 0.044715f * z * z));
-    const float zc = fminf(fmaxf(z, -64.f), 64.f);  // s (1 - s) is 0 beyond: keeps 0 x infinity out
-    return z != z ? z : s + zc * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * zc * zc);
+    // beyond +-64 the derivative is 0 or 1 as there; the limit keeps 0 x infinity out (a NaN stays)
+    const bool nan0 = a != a, nan1 = b != b;
+    const uint64_t z = f2pack(fminf(fmaxf(a, -64.f), 64.f), fminf(fmaxf(b, -64.f), 64.f)), z2 = mul2(z, z);
+    float u0, u1;
+    f2unpack(mul2(fma2(z2, both(-0.10294324f), both(-2.3022082f)), z), u0, u1);
+    f2unpack(add2(f2pack(exp2_fast(u0), exp2_fast(u1)), both(1.f)), u0, u1);
+    const uint64_t s = f2pack(rcp_fast(u0), rcp_fast(u1));
+    const uint64_t w = mul2(mul2(s, z), add2(both(1.f), mul2(s, both(-1.f))));
+    f2unpack(fma2(w, fma2(z2, both(0.21406443f), both(1.5957691f)), s), u0, u1);
+    a = nan0 ? a : u0;
+    b = nan1 ? b : u1;
   } else if constexpr (ACT == FRATTN_ACT_SILU) {
-    const float s = sigmoid_f(z);
-    return s + s * (1.f - s) * z;
+    const uint64_t z = f2pack(a, b);
+    float u0, u1;
+    f2unpack(mul2(z, both(-1.4426950408889634f)), u0, u1);
+    f2unpack(add2(f2pack(exp2_fast(u0), exp2_fast(u1)), both(1.f)), u0, u1);
+    const uint64_t s = f2pack(rcp_fast(u0), rcp_fast(u1));
+    f2unpack(fma2(mul2(s, z), add2(both(1.f), mul2(s, both(-1.f))), s), a, b);
+  } else if constexpr (ACT == FRATTN_ACT_RELU) {
+    a = a > 0.f ? 1.f : (a != a ? a : 0.f);
+    b = b > 0.f ? 1.f : (b != b ? b : 0.f);
   } else {
-    return 1.f;
+    a = b = 1.f;
   }
 }
 

@@ -34,9 +34,10 @@ struct GemmParams {
   int out_w, z_w;              // 4, 2 or 1 elements
   int res_tma;                 // residual read ahead by TMA (16-byte rows, nothing else staged)
   int M, N, nk;                // nk: 64-wide steps of the reduction
+  int a_bytes;                 // of A in a stage (small products)
   int tiles_n, tiles;
   int split;                   // 0: a pair owns whole tiles; else k steps per pair (see Segments)
-  float* partial;              // [2 pairs][256][BN] (split)
+  float* partial;              // [2 pairs][BN / 4][256][4] (split)
   int32_t* status;
   unsigned long long wait_limit_ns;
 };
@@ -221,6 +222,49 @@ __device__ __forceinline__ void add_bias(float (&v)[32], const float* bias) {
   }
 }
 
+// The epilogue of 32 columns [n, n + 32) of a row by one thread, straight to memory (the
+// joined parts of a split product; columns past N hold zeros).
+template <typename T>
+__device__ __forceinline__ void put32(void* base, long long stride, long long row, int n, int N, int width, const float (&v)[32]) {
+  T* dst = static_cast<T*>(base) + row * stride + n;
+  if (width == 8 && n + 32 <= N) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      reinterpret_cast<uint4*>(dst)[c] = make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
+                                                    pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (n + i < N) dst[i] = f32_elem<T>(v[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void finish_row(const GemmParams& p, long long row, int n, float (&v)[32]) {
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (n + i < p.N) v[i] += elem_f32<T>(static_cast<const T*>(p.bias)[n + i]);
+  }
+  if (p.z) put32<T>(p.z, p.z_stride, row, n, p.N, p.z_tma ? 8 : 1, v);
+  if (p.z_codes) {
+    const long long nb = pack_blocks(p.N);
+    uint32_t codes[8];
+    p.z_scales[row * nb + n / 32] = static_cast<uint8_t>(pack32(v, codes));
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      reinterpret_cast<uint4*>(p.z_codes + (row * nb + n / 32) * kPackBlock)[c] =
+          make_uint4(codes[4 * c], codes[4 * c + 1], codes[4 * c + 2], codes[4 * c + 3]);
+  }
+  act_any(p.act, v);
+  if (p.res) {
+    const T* rp = static_cast<const T*>(p.res) + row * p.res_stride + n;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (n + i < p.N) v[i] += elem_f32<T>(rp[i]);
+  }
+  put32<T>(p.out, p.out_stride, row, n, p.N, p.out_tma ? 8 : 1, v);
+}
+
 // GEMM on CTA pairs (cluster of 2, tcgen05 cta_group::2): 256 x BN tiles of D, M = 256
 // MMAs spanning both CTAs, each CTA loading its 128 rows of A and half of the B tile by
 // TMA (128-byte swizzle) into an ST-stage ring, fp32 accumulators in TMEM (two of BN
@@ -402,8 +446,9 @@ __global__ void __launch_bounds__(GemmCfg<BN>::THREADS, 1) gemm_pair_kernel(cons
       }
       const int halves = n + 32 < p.N ? 2 : 1;
       if (!whole) {  // a part of a tile: fp32 sums into the pair's slot
-        float* dst = p.partial + (static_cast<size_t>(2 * pair + (s.k0 ? 0 : 1)) * 256 + 128 * rank + quarter * 32 + lane) * BN +
-                     chunk * 64;
+        // (a lane's row is the fastest index but four columns, so that the lanes write neighbouring 16 bytes)
+        float4* dst = reinterpret_cast<float4*>(p.partial) +
+                      (static_cast<size_t>(2 * pair + (s.k0 ? 0 : 1)) * (BN / 4) + chunk * 16) * 256 + 128 * rank + quarter * 32 + lane;
 #pragma unroll 1
         for (int h = 0; h < halves; ++h) {
           float v[32];
@@ -411,7 +456,7 @@ __global__ void __launch_bounds__(GemmCfg<BN>::THREADS, 1) gemm_pair_kernel(cons
           if (in_row) {
 #pragma unroll
             for (int c = 0; c < 8; ++c)
-              reinterpret_cast<float4*>(dst + 32 * h)[c] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+              dst[(8 * h + c) * 256] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
           }
         }
         release();
@@ -489,86 +534,204 @@ __global__ void __launch_bounds__(GemmCfg<BN>::THREADS, 1) gemm_pair_kernel(cons
   }
 }
 
-// Joins the parts of split tiles in the order of k and applies the epilogue: eight
-// columns of a row per thread, four neighbouring threads a block of 32 columns.
+// Joins the parts of split tiles in the order of k and applies the epilogue: 32 columns
+// of a row per thread, the rows of a warp's threads neighbours.
 template <int BN, typename T>
 __global__ void __launch_bounds__(256) gemm_finish_kernel(const __grid_constant__ GemmParams p) {
   const int t = blockIdx.x;
   const int first = static_cast<int>(static_cast<long long>(t) * p.nk / p.split);
   const int last = static_cast<int>((static_cast<long long>(t + 1) * p.nk - 1) / p.split);
   if (first == last) return;  // one pair computed the whole tile
-  const int m0 = (t / p.tiles_n) * 256, n0 = (t % p.tiles_n) * BN;
-  const long long nb = pack_blocks(p.N);
-  constexpr int PER_ROW = BN / 8;
-  constexpr int ROWS = 256 / PER_ROW;  // rows of one pass of the block
-  const int c = static_cast<int>(threadIdx.x) % PER_ROW * 8, n = n0 + c;
-  for (int r = blockIdx.y * ROWS + static_cast<int>(threadIdx.x) / PER_ROW; r < 256; r += gridDim.y * ROWS) {
-    const long long row = m0 + r;
-    if (m0 + r - static_cast<int>(threadIdx.x) / PER_ROW >= p.M) break;  // (the same for the whole block)
-    const bool in = row < p.M && n < p.N;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (in) {
-      for (int q = first; q <= last; ++q) {
-        const long long b = static_cast<long long>(q) * p.split;
-        const int slot = 2 * q + (b > static_cast<long long>(t) * p.nk ? 0 : 1);  // began inside the tile, or before or at its first step
-        const float4* src = reinterpret_cast<const float4*>(p.partial + (static_cast<size_t>(slot) * 256 + r) * BN + c);
-        const float4 x = __ldcg(src), y = __ldcg(src + 1);
-        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
-      }
-    }
+  const int unit = blockIdx.y * 8 + static_cast<int>(threadIdx.x >> 5);  // of 32 rows x 32 columns
+  const int r = unit % 8 * 32 + static_cast<int>(threadIdx.x & 31), c = unit / 8 * 32;
+  const long long row = static_cast<long long>(t / p.tiles_n) * 256 + r;
+  const int n = (t % p.tiles_n) * BN + c;
+  if (row >= p.M || n >= p.N) return;
+  float v[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = 0.f;
+  for (int q = first; q <= last; ++q) {
+    const long long b = static_cast<long long>(q) * p.split;
+    const int slot = 2 * q + (b > static_cast<long long>(t) * p.nk ? 0 : 1);  // began inside the tile, or before or at its first step
+    const float4* src = reinterpret_cast<const float4*>(p.partial) + (static_cast<size_t>(slot) * (BN / 4) + c / 4) * 256 + r;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (in && n + i < p.N) {
-        if (p.bias) v[i] += elem_f32<T>(static_cast<const T*>(p.bias)[n + i]);
-      } else {
-        v[i] = 0.f;
+      const float4 x = __ldcg(src + i * 256);
+      v[4 * i] += x.x;
+      v[4 * i + 1] += x.y;
+      v[4 * i + 2] += x.z;
+      v[4 * i + 3] += x.w;
+    }
+  }
+  finish_row<T>(p, row, n, v);
+}
+
+// ------------------------------------------------------------------ small products
+// One CTA per 128 x 64 tile of D, and per cluster of S CTAs one tile: each of the S takes
+// a share of the reduction, so that a product of few rows (a single token reads W and
+// little else) or a short one still has every SM loading, with all of a CTA's steps on
+// their way at once. The S sums meet through distributed shared memory, in the order
+// of the ranks, and each CTA finishes a part of the tile. No second kernel, no sums in
+// global memory.
+struct SmallCfg {
+  static constexpr int BM = 128, BN = 64, BK = 64;
+  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES;
+  static constexpr int ST = 4;
+  static constexpr int SUM_BYTES = BM * BN * 4;  // this CTA's sums, over the first stages' place
+  static constexpr int OFF_BAR = ST * STAGE;
+  static constexpr int SMEM = OFF_BAR + 128 + 1024;
+  static constexpr int THREADS = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+  static_assert(SUM_BYTES <= ST * STAGE, "sums fit");
+};
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+
+template <bool AMN, bool BMN, typename T>
+__global__ void __launch_bounds__(SmallCfg::THREADS) gemm_small_kernel(const __grid_constant__ GemmParams p) {
+  using C = SmallCfg;
+  constexpr int ST = C::ST;
+  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t IDESC = make_idesc_f16(kBF16, C::BM, C::BN, BMN) | (AMN ? 1u << 15 : 0u);
+  constexpr uint32_t SW128 = 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+  const int FULL = 0, EMPTY = ST, ACC = 2 * ST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = p.split, rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int tile = static_cast<int>(blockIdx.x) / S;
+  const int m0 = (tile / p.tiles_n) * C::BM, n0 = (tile % p.tiles_n) * C::BN;
+  const int k0 = static_cast<int>(static_cast<long long>(p.nk) * rank / S), k1 = static_cast<int>(static_cast<long long>(p.nk) * (rank + 1) / S);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(bar(FULL + i), 1);
+      mbar_init(bar(EMPTY + i), 1);
+    }
+    mbar_init(bar(ACC), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&p.tma_a);
+    tma_prefetch_desc(&p.tma_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 64);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int st = it % ST;
+        if (!gemm_wait(bar(EMPTY + st), ((it / ST) & 1) ^ 1, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x76)) break;
+        const uint32_t a = smem_u32(smem + st * C::STAGE), b = a + C::A_BYTES;
+        mbar_arrive_expect_tx(bar(FULL + st), p.a_bytes + C::B_BYTES);
+        if constexpr (AMN) {
+          tma_load_2d(a, &p.tma_a, bar(FULL + st), m0, kb * C::BK);
+          tma_load_2d(a + 8192, &p.tma_a, bar(FULL + st), m0 + 64, kb * C::BK);
+        } else {  // (boxes of as many rows as M has; the rest of the tile's rows go nowhere)
+          tma_load_2d(a, &p.tma_a, bar(FULL + st), kb * C::BK, m0);
+        }
+        if constexpr (BMN) tma_load_2d(b, &p.tma_b, bar(FULL + st), n0, kb * C::BK);
+        else tma_load_2d(b, &p.tma_b, bar(FULL + st), kb * C::BK, n0);
+      }
+      for (int i = it > ST ? it - ST : 0; i < it; ++i) gemm_drain(bar(FULL + i % ST), (i / ST) & 1, p.wait_limit_ns);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int it = 0;
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int st = it % ST;
+        if (!gemm_wait(bar(FULL + st), (it / ST) & 1, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x77)) break;
+        tc_fence_after();
+        const uint32_t a = smem_u32(smem + st * C::STAGE);
+        const uint64_t ad = make_sdesc(a, AMN ? 8192 : 16, 1024, SW128);
+        const uint64_t bd = make_sdesc(a + C::A_BYTES, BMN ? 8192 : 16, 1024, SW128);
+#pragma unroll
+        for (int kk = 0; kk < C::BK / 16; ++kk)
+          umma_ss(tmem, ad + (AMN ? 128 : 2) * kk, bd + (BMN ? 128 : 2) * kk, IDESC, it | kk);
+        umma_commit(bar(EMPTY + st));
+      }
+      umma_commit(bar(ACC));  // (after a timeout too: it then only says that the MMAs issued are done)
+      gemm_drain(bar(ACC), 0, p.wait_limit_ns);
+    }
+  }
+  __syncwarp();
+  const int quarter = warp & 3;
+  const bool rows = warp >= 2 && m0 + quarter * 32 < p.M;  // an epilogue warp with rows of D
+  const long long row = m0 + quarter * 32 + lane;
+  bool ok = true;
+  if (rows) {
+    ok = __all_sync(0xffffffffu, gemm_wait(bar(ACC), 0, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x78));
+    tc_fence_after();
+  }
+  const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  if (S == 1) {
+    if (rows && ok) {
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        if (n0 + 32 * h >= p.N) break;
+        float v[32];
+        tmem_ld32(acc + 32 * h, reinterpret_cast<uint32_t (&)[32]>(v));
+        tmem_ld_wait();
+        if (row < p.M) finish_row<T>(p, row, n0 + 32 * h, v);
       }
     }
-    if (p.z_codes) {
-      uint32_t m = 0;
+  } else {
+    // (the stages' place: all MMAs, the stages' readers, are done when ACC has completed)
+    float4* sums = reinterpret_cast<float4*>(smem);  // [16 groups of 4 columns][128 rows]
+    if (rows && ok) {
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        float v[32];
+        tmem_ld32(acc + 32 * h, reinterpret_cast<uint32_t (&)[32]>(v));
+        tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const uint32_t sc = pack_scale(m);
-      const float inv = pack_inv(sc), lim = pack_limit(sc);
-      if (row < p.M && n < nb * kPackBlock) {
-        uint2 w;
-        w.x = pack_code4(v[0], v[1], v[2], v[3], inv, lim);
-        w.y = pack_code4(v[4], v[5], v[6], v[7], inv, lim);
-        *reinterpret_cast<uint2*>(p.z_codes + row * nb * kPackBlock + n) = w;
-        if (n % kPackBlock == 0) p.z_scales[row * nb + n / kPackBlock] = static_cast<uint8_t>(sc);
+        for (int c = 0; c < 8; ++c)
+          sums[(8 * h + c) * 128 + quarter * 32 + lane] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
       }
     }
-    if (!in) continue;
-    float y[8];
+    cluster_sync_all();  // every CTA's sums are written (a CTA without rows or timed out has none to read)
+    // this CTA's share of the tile's (row, 32 columns) units
+    if (warp >= 2) {
+      const int share = 256 / S, t = (warp - 2) * 32 + lane;
+      for (int u = rank * share + t; u < (rank + 1) * share; u += 128) {
+        const int r = u & 127, h = u >> 7, n = n0 + 32 * h;
+        if (m0 + r >= p.M || n >= p.N) continue;
+        float v[32];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = v[i];
-    act_any(p.act, y);
-    if (p.res) {
-      const T* rp = static_cast<const T*>(p.res) + row * p.res_stride + n;
+        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        for (int q = 0; q < S; ++q) {
+          const uint32_t from = mapa_shared(smem_u32(sums + (8 * h) * 128 + r), q);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (n + i < p.N) y[i] += elem_f32<T>(rp[i]);
-    }
-    auto put = [&](void* base, long long stride, const float (&f)[8], int wide) {
-      T* dst = static_cast<T*>(base) + row * stride + n;
-      if (wide) {
-        uint4 w;
-        w.x = pack2<T>(f[0], f[1]);
-        w.y = pack2<T>(f[2], f[3]);
-        w.z = pack2<T>(f[4], f[5]);
-        w.w = pack2<T>(f[6], f[7]);
-        *reinterpret_cast<uint4*>(dst) = w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (n + i < p.N) dst[i] = f32_elem<T>(f[i]);
+          for (int c = 0; c < 8; ++c) {
+            const float4 x = ld_cluster_f4(from + c * 128 * 16);
+            v[4 * c] += x.x;
+            v[4 * c + 1] += x.y;
+            v[4 * c + 2] += x.z;
+            v[4 * c + 3] += x.w;
+          }
+        }
+        finish_row<T>(p, m0 + r, n, v);
       }
-    };
-    if (p.z) put(p.z, p.z_stride, v, p.z_tma && n + 8 <= p.N);
-    put(p.out, p.out_stride, y, p.out_tma && n + 8 <= p.N);
+    }
+    cluster_sync_all();  // nobody leaves while its sums may be read
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 64);
   }
 }
 
@@ -617,7 +780,7 @@ int sm_pairs() {
 
 // Tile width and split of an M x N product over nk steps of 64.
 struct GemmPlan {
-  int bn, tiles, split, pairs;
+  int bn, tiles, split, pairs;  // bn 64: the small kernel, split its CTAs per tile
   size_t partial_bytes;
 };
 
@@ -632,13 +795,26 @@ GemmPlan gemm_plan(int M, int N, int nk) {
   GemmPlan best{};
   const int P = sm_pairs();
   double best_us = 1e30;
+  {
+    // 128 x 64 tiles, up to 8 CTAs on one while that leaves each two steps and two CTAs to
+    // an SM: bound by 24 KB from L2 a step (10 TB/s for all), or by latency
+    const long long tiles = static_cast<long long>((M + 127) / 128) * ((N + 63) / 64);
+    int S = 1;
+    while (S < 8 && tiles * 2 * S <= 4 * P && nk >= 4 * S) S *= 2;
+    const double rows = M < 128 ? M : 128;
+    const double us = tiles * nk * (rows * 128 + 8192) / 10e6 + 0.25 * ((nk + S - 1) / S) * ((tiles * S + 4 * P - 1) / (4 * P)) + 1.0;
+    if (tiles * S < (1 << 30)) {
+      best_us = us;
+      best = GemmPlan{64, static_cast<int>(tiles), S, 0, 0};
+    }
+  }
   for (int bn : {256, 128}) {
     const long long tiles = static_cast<long long>((M + 255) / 256) * ((N + bn - 1) / bn);
     if (tiles > (1 << 30) / (nk + 1)) continue;
     const double step_us = bn == 256 ? 0.37 : 0.31;
     {
       const long long rounds = (tiles + P - 1) / P;
-      const double us = static_cast<double>(rounds) * nk * step_us;
+      const double us = static_cast<double>(rounds) * nk * step_us + 4.0;  // (filling, the last tile's epilogue)
       if (us < best_us) {
         best_us = us;
         best = GemmPlan{bn, static_cast<int>(tiles), 0, static_cast<int>(tiles < P ? tiles : P), 0};
@@ -650,7 +826,7 @@ GemmPlan gemm_plan(int M, int N, int nk) {
     if (tiles % P != 0) {
       const int pairs = static_cast<int>((total + split - 1) / split);
       const double rows = M < 256 ? M : 256;
-      const double us = split * step_us + 4.0 + 2.0 * pairs * rows * bn * 4 * 2 / 4e6;
+      const double us = split * step_us + 8.0 + 2.0 * pairs * rows * bn * 4 * 2 / 4e6;
       if (us < best_us) {
         best_us = us;
         best = GemmPlan{bn, static_cast<int>(tiles), split, pairs, static_cast<size_t>(2) * pairs * 256 * bn * 4};
@@ -686,7 +862,35 @@ int gemm_launch(GemmParams& p, const GemmPlan& plan, cudaStream_t st) {
   lc.attrs = &attr;
   lc.numAttrs = 1;
   if (cudaLaunchKernelEx(&lc, kern, p) != cudaSuccess) return FRATTN_E_CUDA;
-  if (plan.split) gemm_finish_kernel<BN, T><<<dim3(plan.tiles, 8), 256, 0, st>>>(p);
+  if (plan.split) gemm_finish_kernel<BN, T><<<dim3(plan.tiles, BN / 32), 256, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? 0 : FRATTN_E_CUDA;
+}
+
+template <bool AMN, bool BMN, typename T>
+int gemm_small_launch(const GemmParams& p, const GemmPlan& plan, cudaStream_t st) {
+  auto kern = gemm_small_kernel<AMN, BMN, T>;
+  static unsigned long long attr_set = 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bitv = 1ull << (dev & 63);
+  if (!(attr_set & bitv)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SmallCfg::SMEM) != cudaSuccess)
+      return FRATTN_E_CUDA;
+    attr_set |= bitv;
+  }
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = plan.split;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(plan.tiles * plan.split);
+  lc.blockDim = dim3(SmallCfg::THREADS);
+  lc.dynamicSmemBytes = SmallCfg::SMEM;
+  lc.stream = st;
+  lc.attrs = &attr;
+  lc.numAttrs = 1;
+  if (cudaLaunchKernelEx(&lc, kern, p) != cudaSuccess) return FRATTN_E_CUDA;
   return cudaGetLastError() == cudaSuccess ? 0 : FRATTN_E_CUDA;
 }
 
@@ -708,8 +912,11 @@ int gemm(GemmParams& p, const Mat& a, const Mat& b, int M, int N, int K, void* w
   p.partial = static_cast<float*>(ws);
   p.status = status;
   p.wait_limit_ns = frattn_wait_limit_ns();
-  if (encode_map(&p.tma_a, a.p, AMN ? M : K, AMN ? K : M, a.stride, 64, AMN ? 64 : 128, bf16) ||
-      encode_map(&p.tma_b, b.p, BMN ? N : K, BMN ? K : N, b.stride, 64, BMN ? 64 : plan.bn / 2, bf16))
+  const bool small = plan.bn == 64;
+  const int a_rows = small && M < 128 ? (M + 7) / 8 * 8 : 128;  // of a K-major A in a box
+  p.a_bytes = AMN ? SmallCfg::A_BYTES : a_rows * 128;
+  if (encode_map(&p.tma_a, a.p, AMN ? M : K, AMN ? K : M, a.stride, 64, AMN ? 64 : a_rows, bf16) ||
+      encode_map(&p.tma_b, b.p, BMN ? N : K, BMN ? K : N, b.stride, 64, BMN || small ? 64 : plan.bn / 2, bf16))
     return FRATTN_E_TMAP;
   auto width = [&](const void* q, long long stride) {
     for (int w = 4; w > 1; w >>= 1)
@@ -718,13 +925,14 @@ int gemm(GemmParams& p, const Mat& a, const Mat& b, int M, int N, int K, void* w
   };
   p.out_tma = rows16(p.out, p.out_stride);
   p.out_w = width(p.out, p.out_stride);
-  if (p.out_tma && encode_map(&p.tma_out, p.out, N, M, p.out_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
+  if (p.out_tma && !small && encode_map(&p.tma_out, p.out, N, M, p.out_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
   if (p.z) {
     p.z_tma = rows16(p.z, p.z_stride);
     p.z_w = width(p.z, p.z_stride);
-    if (p.z_tma && encode_map(&p.tma_z, p.z, N, M, p.z_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
+    if (p.z_tma && !small && encode_map(&p.tma_z, p.z, N, M, p.z_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
   }
-  if (p.z_codes && encode_codes_map(&p.tma_codes, p.z_codes, pack_blocks(N) * kPackBlock, M)) return FRATTN_E_TMAP;
+  if (p.z_codes && !small && encode_codes_map(&p.tma_codes, p.z_codes, pack_blocks(N) * kPackBlock, M)) return FRATTN_E_TMAP;
+  if (small) return gemm_small_launch<AMN, BMN, T>(p, plan, st);
   p.res_tma = p.res && rows16(p.res, p.res_stride) && p.res_stride >= N && !p.z && !p.z_codes;
   if (p.res_tma && encode_map(&p.tma_res, p.res, N, M, p.res_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
   if (plan.bn == 256) return gemm_launch<256, AMN, BMN, T>(p, plan, st);
@@ -791,7 +999,13 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
         if constexpr (PACKED) q[r].get(pack_step(scale[r]), f);
         else z[r].get(f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) d[e] *= act_grad_f<ACT>(f[e]);
+        for (int e = 0; e + 1 < VEC; e += 2) act_grad_f2<ACT>(f[e], f[e + 1]);
+        if constexpr (VEC == 1) {
+          float none = 0.f;
+          act_grad_f2<ACT>(f[0], none);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[e] *= f[e];
       }
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sum[e] += d[e];
@@ -804,7 +1018,10 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
   }
 }
 
-constexpr int kMaxStrips = 592;  // partial rows of the bias gradient
+// Strips of rows, and partial rows of the bias gradient: two blocks of 256 threads to an
+// SM with four rows each on their way are enough for the memory, and more strips cost
+// more partial sums (592 of them took 8 us to add up at N = 3424).
+constexpr int kMaxStrips = 296;
 
 template <typename T, int VEC, int ACT, bool PACKED>
 int act_bwd_launch(const ActBwdParams& p, int* groups, cudaStream_t st) {
@@ -812,7 +1029,7 @@ int act_bwd_launch(const ActBwdParams& p, int* groups, cudaStream_t st) {
   const int tiles = (nv + 255) / 256;
   const int bx = ((nv + tiles - 1) / tiles + 31) / 32 * 32;
   const int gx = (nv + bx - 1) / bx;
-  long long gy = static_cast<long long>(sm_count_for_current_device()) * 8 / gx;
+  long long gy = static_cast<long long>(sm_count_for_current_device()) * (512 / bx) / gx;
   const long long rows4 = (p.T + 3) / 4;
   if (gy > rows4) gy = rows4;
   if (gy > kMaxStrips) gy = kMaxStrips;
