@@ -59,7 +59,7 @@ struct Vec {
   uint32_t w[kParts * kPartWords];
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) raw_words(__ldg(reinterpret_cast<const Raw*>(p) + i), w + i * kPartWords);
+    for (int i = 0; i < kParts; ++i) raw_words(__ldcg(reinterpret_cast<const Raw*>(p) + i), w + i * kPartWords);
   }
   __device__ __forceinline__ void get(float (&v)[VEC]) const {
     if constexpr (std::is_same<T, float>::value) {
@@ -101,7 +101,7 @@ struct CodeVec {
   static constexpr int kWords = VEC < 4 ? 1 : VEC / 4;
   uint32_t w[kWords];
   __device__ __forceinline__ void load(const int8_t* p) {
-    raw_words(__ldg(reinterpret_cast<const typename RawVec<VEC>::type*>(p)), w);
+    raw_words(__ldcg(reinterpret_cast<const typename RawVec<VEC>::type*>(p)), w);
   }
   __device__ __forceinline__ void get(float step, float (&v)[VEC]) const {
 #pragma unroll
@@ -128,6 +128,33 @@ struct RowVec {
     return *this;
   }
 };
+
+// Launch whose start overlaps the end of the kernel before it in the stream (programmatic
+// dependent launch): the block operators are short, and follow each other. Every kernel
+// launched this way executes griddep_wait() before its first access to global memory
+// (it waits until the kernels before have completed and their writes are visible), and
+// griddep_launch_dependents() once it has nothing left to set up. Its loads go to L2
+// (ld.global.cg) or through the asynchronous copies, never through the non-coherent path,
+// whose lines may be older than the writes waited for.
+template <typename... P, typename... A>
+inline int launch_overlapped(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, A... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = grid;
+  lc.blockDim = block;
+  lc.dynamicSmemBytes = smem;
+  lc.stream = st;
+  lc.attrs = attr;
+  lc.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&lc, kern, static_cast<P>(args)...);
+  return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : FRATTN_E_CUDA;
+}
 
 inline bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 

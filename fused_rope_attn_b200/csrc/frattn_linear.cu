@@ -319,6 +319,8 @@ __global__ void __launch_bounds__(GemmCfg<BN>::THREADS, 1) gemm_pair_kernel(cons
   cluster_sync_all();  // barriers of both CTAs initialised, TMEM allocated
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -541,11 +543,16 @@ __global__ void __launch_bounds__(256) gemm_finish_kernel(const __grid_constant_
   const int t = blockIdx.x;
   const int first = static_cast<int>(static_cast<long long>(t) * p.nk / p.split);
   const int last = static_cast<int>((static_cast<long long>(t + 1) * p.nk - 1) / p.split);
-  if (first == last) return;  // one pair computed the whole tile
+  if (first == last) {  // one pair computed the whole tile
+    griddep_wait();
+    return;
+  }
   const int unit = blockIdx.y * 8 + static_cast<int>(threadIdx.x >> 5);  // of 32 rows x 32 columns
   const int r = unit % 8 * 32 + static_cast<int>(threadIdx.x & 31), c = unit / 8 * 32;
   const long long row = static_cast<long long>(t / p.tiles_n) * 256 + r;
   const int n = (t % p.tiles_n) * BN + c;
+  griddep_wait();
+  griddep_launch_dependents();
   if (row >= p.M || n >= p.N) return;
   float v[32];
 #pragma unroll
@@ -628,6 +635,8 @@ __global__ void __launch_bounds__(SmallCfg::THREADS) gemm_small_kernel(const __g
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
   if (warp == 0) {
     if (lane == 0) {
       int it = 0;
@@ -849,21 +858,9 @@ int gemm_launch(GemmParams& p, const GemmPlan& plan, cudaStream_t st) {
       return FRATTN_E_CUDA;
     attr_set |= bitv;
   }
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 2;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(2 * plan.pairs);
-  lc.blockDim = dim3(C::THREADS);
-  lc.dynamicSmemBytes = C::SMEM;
-  lc.stream = st;
-  lc.attrs = &attr;
-  lc.numAttrs = 1;
-  if (cudaLaunchKernelEx(&lc, kern, p) != cudaSuccess) return FRATTN_E_CUDA;
-  if (plan.split) gemm_finish_kernel<BN, T><<<dim3(plan.tiles, BN / 32), 256, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? 0 : FRATTN_E_CUDA;
+  const int rc = launch_overlapped(kern, dim3(2 * plan.pairs), dim3(C::THREADS), C::SMEM, st, 2, p);
+  if (rc || !plan.split) return rc;
+  return launch_overlapped(gemm_finish_kernel<BN, T>, dim3(plan.tiles, BN / 32), dim3(256), 0, st, 1, p);
 }
 
 template <bool AMN, bool BMN, typename T>
@@ -878,20 +875,7 @@ int gemm_small_launch(const GemmParams& p, const GemmPlan& plan, cudaStream_t st
       return FRATTN_E_CUDA;
     attr_set |= bitv;
   }
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = plan.split;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(plan.tiles * plan.split);
-  lc.blockDim = dim3(SmallCfg::THREADS);
-  lc.dynamicSmemBytes = SmallCfg::SMEM;
-  lc.stream = st;
-  lc.attrs = &attr;
-  lc.numAttrs = 1;
-  if (cudaLaunchKernelEx(&lc, kern, p) != cudaSuccess) return FRATTN_E_CUDA;
-  return cudaGetLastError() == cudaSuccess ? 0 : FRATTN_E_CUDA;
+  return launch_overlapped(kern, dim3(plan.tiles * plan.split), dim3(SmallCfg::THREADS), SmallCfg::SMEM, st, plan.split, p);
 }
 
 // D[M, N] = A B^T with the epilogue in p (bias .. z_scales set by the caller). A is
@@ -962,6 +946,8 @@ template <typename T, int VEC, int ACT, bool PACKED>
 __global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
   constexpr int R = 4;
   const int v = blockIdx.x * blockDim.x + threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
   if (v * VEC >= p.N) return;
   const size_t c = static_cast<size_t>(v) * VEC;
   const int nb = static_cast<int>(pack_blocks(p.N));
@@ -981,7 +967,7 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
         if constexpr (ACT != FRATTN_ACT_NONE) {
           if constexpr (PACKED) {
             q[r].load(p.z_codes + row * nb * kPackBlock + c);
-            scale[r] = __ldg(p.z_scales + row * nb + v * VEC / kPackBlock);
+            scale[r] = __ldcg(p.z_scales + row * nb + v * VEC / kPackBlock);
           } else {
             z[r].load(static_cast<const T*>(p.z) + row * p.z_stride + c);
           }
@@ -1035,8 +1021,7 @@ int act_bwd_launch(const ActBwdParams& p, int* groups, cudaStream_t st) {
   if (gy > kMaxStrips) gy = kMaxStrips;
   if (gy < 1) gy = 1;
   *groups = static_cast<int>(gy);
-  act_bwd_kernel<T, VEC, ACT, PACKED><<<dim3(gx, static_cast<unsigned>(gy)), bx, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? 0 : FRATTN_E_CUDA;
+  return launch_overlapped(act_bwd_kernel<T, VEC, ACT, PACKED>, dim3(gx, static_cast<unsigned>(gy)), dim3(bx), 0, st, 1, p);
 }
 
 template <typename T, int VEC, bool PACKED>

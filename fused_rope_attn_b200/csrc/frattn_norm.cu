@@ -72,7 +72,7 @@ __device__ __forceinline__ void block_sum(float (&s)[R], float* red) {
 
 __device__ __forceinline__ float param_at(const void* p, int f32, int dtype_bf16, int c, float fill) {
   if (!p) return fill;
-  if (f32) return __ldg(static_cast<const float*>(p) + c);
+  if (f32) return __ldcg(static_cast<const float*>(p) + c);
   return dtype_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[c]) : __half2float(static_cast<const __half*>(p)[c]);
 }
 
@@ -266,7 +266,7 @@ __device__ __forceinline__ void stage_param(float* to, const void* src, int f32,
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int at = c + e < C ? c + e : C - 1;  // (past C: any value, the gradient there is 0)
-        v[e] = f32 ? __ldg(static_cast<const float*>(src) + at) : elem_f32<T>(static_cast<const T*>(src)[at]);
+        v[e] = f32 ? __ldcg(static_cast<const float*>(src) + at) : elem_f32<T>(static_cast<const T*>(src)[at]);
       }
     }
 #pragma unroll
@@ -303,7 +303,7 @@ __device__ __forceinline__ void unit_param_global(const void* p, int f32, int ve
         r.get(x);
       } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x[e] = c < C ? __ldg(src + e) : 0.f;
+        for (int e = 0; e < VEC; ++e) x[e] = c < C ? __ldcg(src + e) : 0.f;
       }
     });
   } else {
@@ -327,6 +327,8 @@ __global__ void __launch_bounds__(256) layer_norm_fwd_few_kernel(const NormParam
   __shared__ float red[1][2][8];
   const Team team(blockDim.x / 32);
   const long long row = blockIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
   const int c0 = lane_col<VEC, NU>(team), full = full_units<NU>(team, p.C);
   const T* src = static_cast<const T*>(p.x) + row * p.x_stride;
   float x[NU][8], s[1] = {0.f};
@@ -400,6 +402,8 @@ __global__ void __launch_bounds__(256, NU > 3 ? 3 : 4) layer_norm_fwd_kernel(con
   };
   for (int k = 0; k < l.passes; ++k) clear_tail(ring + k * l.slot, bytes, l.slot, team);
   team.sync();
+  griddep_wait();
+  griddep_launch_dependents();
   for (int k = 0; k < l.passes - 1; ++k) fetch();
   stage_param<T, VEC>(w, p.w, p.w_f32, 1.f, p.C, l.cols);
   stage_param<T, VEC>(b, p.b, p.w_f32, 0.f, p.C, l.cols);
@@ -458,6 +462,8 @@ __global__ void __launch_bounds__(256, NU > 3 ? 3 : 4) layer_norm_fwd_kernel(con
 // (from L2 after the first).
 template <typename T>
 __global__ void __launch_bounds__(1024) layer_norm_fwd_wide_kernel(const NormParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   __shared__ float red[2][32];
   const float inv_c = 1.f / static_cast<float>(p.C);
@@ -522,6 +528,7 @@ __global__ void __launch_bounds__(384) layer_norm_bwd_kernel(const NormParams p,
     if constexpr (PACKED) clear_tail(slot + off_s, nb, l.slot - off_s, team);
   }
   team.sync();
+  griddep_wait();
   for (int k = 0; k < l.passes - 1; ++k) fetch();
   stage_param<T, VEC>(w, p.w, p.w_f32, 1.f, p.C, l.cols);
   __syncthreads();
@@ -531,13 +538,13 @@ __global__ void __launch_bounds__(384) layer_norm_bwd_kernel(const NormParams p,
   for (int u = 0; u < NU; ++u)
 #pragma unroll
     for (int e = 0; e < 4; ++e) dw[u][e] = db[u][e] = 0;
-  float nmean = first < p.T ? __ldg(p.mean + first) : 0.f, nrstd = first < p.T ? __ldg(p.rstd + first) : 0.f;
+  float nmean = first < p.T ? __ldcg(p.mean + first) : 0.f, nrstd = first < p.T ? __ldcg(p.rstd + first) : 0.f;
   int at = 0;
   for (long long row = first; row < p.T; row += step) {
     const float mean = nmean, rstd = nrstd;
     if (row + step < p.T) {
-      nmean = __ldg(p.mean + row + step);
-      nrstd = __ldg(p.rstd + row + step);
+      nmean = __ldcg(p.mean + row + step);
+      nrstd = __ldcg(p.rstd + row + step);
     }
     if (l.passes == 2) copies_wait<0>();
     else copies_wait<1>();
@@ -614,7 +621,6 @@ __global__ void __launch_bounds__(384) layer_norm_bwd_kernel(const NormParams p,
     at = at + 1 == l.passes ? 0 : at + 1;
   }
   if (!p.partial) return;
-  griddep_launch_dependents();
   // the block's teams add their columns' sums: each in its own part of shared memory
   copies_wait<0>();
   __syncthreads();
@@ -647,7 +653,7 @@ template <typename T, bool PACKED>
 __device__ __forceinline__ float wide_x(const NormParams& p, long long row, int c) {
   if constexpr (PACKED) {
     const long long nb = pack_blocks(p.C);
-    return static_cast<float>(__ldg(p.codes + row * nb * kPackBlock + c)) * pack_step(__ldg(p.scales + row * nb + c / kPackBlock));
+    return static_cast<float>(__ldcg(p.codes + row * nb * kPackBlock + c)) * pack_step(__ldcg(p.scales + row * nb + c / kPackBlock));
   } else {
     return elem_f32<T>(static_cast<const T*>(p.x)[row * p.x_stride + c]);
   }
@@ -655,12 +661,14 @@ __device__ __forceinline__ float wide_x(const NormParams& p, long long row, int 
 
 template <typename T, bool PACKED>
 __global__ void __launch_bounds__(1024) layer_norm_bwd_wide_kernel(const NormParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   __shared__ float red[2][64];
   const float inv_c = 1.f / static_cast<float>(p.C);
   int phase = 0;
   for (long long row = blockIdx.x; row < p.T; row += gridDim.x, phase ^= 1) {
-    const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
+    const float mean = __ldcg(p.mean + row), rstd = __ldcg(p.rstd + row);
     const T* dy = static_cast<const T*>(p.dy) + row * p.dy_stride;
     T* out = static_cast<T*>(p.out) + row * p.out_stride;
     float s[2] = {0.f, 0.f};
@@ -680,12 +688,14 @@ __global__ void __launch_bounds__(1024) layer_norm_bwd_wide_kernel(const NormPar
 
 template <typename T, bool PACKED>
 __global__ void __launch_bounds__(256) layer_norm_bwd_wide_cols_kernel(const NormParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
   const int c = blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= p.C) return;
   float dw = 0.f, db = 0.f;
   for (long long row = blockIdx.y; row < p.T; row += gridDim.y) {
     const float d = elem_f32<T>(static_cast<const T*>(p.dy)[row * p.dy_stride + c]);
-    dw += d * (wide_x<T, PACKED>(p, row, c) - __ldg(p.mean + row)) * __ldg(p.rstd + row);
+    dw += d * (wide_x<T, PACKED>(p, row, c) - __ldcg(p.mean + row)) * __ldcg(p.rstd + row);
     db += d;
   }
   p.partial[static_cast<size_t>(blockIdx.y) * 2 * p.C + c] = dw;
@@ -706,6 +716,7 @@ __global__ void __launch_bounds__(1024) column_finish_kernel(const FinishParams 
   __shared__ float red[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x, a = blockIdx.y;
   griddep_wait();
+  griddep_launch_dependents();
   float s = 0.f;
   if (c < p.C)
 #pragma unroll 8
@@ -744,6 +755,8 @@ __global__ void __launch_bounds__(256) act_pack_kernel(const PackParams p) {
   constexpr int R = 4;
   const int nb = static_cast<int>(pack_blocks(p.C));
   const int v = blockIdx.x * blockDim.x + threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
   const bool in_row = v < nb * G;  // uniform within a block of 32 values
   const bool has = v * VEC < p.C;
   const long long step = static_cast<long long>(gridDim.y) * blockDim.y;
@@ -791,6 +804,8 @@ __global__ void __launch_bounds__(256) act_unpack_kernel(const PackParams p) {
   constexpr int R = 4;
   const int nb = static_cast<int>(pack_blocks(p.C));
   const int v = blockIdx.x * blockDim.x + threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
   if (v * VEC >= p.C) return;
   const long long step = static_cast<long long>(gridDim.y) * blockDim.y;
   for (long long row0 = static_cast<long long>(blockIdx.y) * blockDim.y + threadIdx.y; row0 < p.T; row0 += step * R) {
@@ -801,7 +816,7 @@ __global__ void __launch_bounds__(256) act_unpack_kernel(const PackParams p) {
       const long long row = row0 + r * step;
       if (row < p.T) {
         in[r].load(p.codes + row * nb * kPackBlock + static_cast<size_t>(v) * VEC);
-        scale[r] = __ldg(p.scales + row * nb + v * VEC / kPackBlock);
+        scale[r] = __ldcg(p.scales + row * nb + v * VEC / kPackBlock);
       }
     }
 #pragma unroll
@@ -819,8 +834,6 @@ int sms() {
   const int n = sm_count_for_current_device();
   return n > 0 ? n : 148;
 }
-
-int launched() { return cudaGetLastError() == cudaSuccess ? 0 : FRATTN_E_CUDA; }
 
 constexpr int kMaxCols = 8192;  // widest row held in registers (8 warps of 1024 columns)
 
@@ -914,8 +927,7 @@ template <typename T>
 int norm_fwd(NormParams p, cudaStream_t st) {
   if (p.C > kMaxCols) {
     const int n = p.T < 2 * sms() ? p.T : 2 * sms();
-    layer_norm_fwd_wide_kernel<T><<<n, 1024, 0, st>>>(p);
-    return launched();
+    return launch_overlapped(layer_norm_fwd_wide_kernel<T>, dim3(n), dim3(1024), 0, st, 1, p);
   }
   RowVec rv(p.C, sizeof(T));
   rv.row(p.x, p.x_stride).row(p.out, p.out_stride);
@@ -923,8 +935,8 @@ int norm_fwd(NormParams p, cudaStream_t st) {
     p.w_vec = aligned_to(p.w, 16) && aligned_to(p.b, 16);
     const int warps = short_team_warps(p.C);
     return with_shape(rv.v, p.C, warps, [&](auto vec, auto nu) {
-      layer_norm_fwd_few_kernel<T, decltype(vec)::value, decltype(nu)::value><<<p.T, 32 * warps, 0, st>>>(p);
-      return launched();
+      return launch_overlapped(layer_norm_fwd_few_kernel<T, decltype(vec)::value, decltype(nu)::value>, dim3(p.T),
+                               dim3(32 * warps), 0, st, 1, p);
     });
   }
   const int warps = team_warps(p.C, rv.v);
@@ -935,8 +947,8 @@ int norm_fwd(NormParams p, cudaStream_t st) {
     auto kern = layer_norm_fwd_kernel<T, decltype(vec)::value, decltype(nu)::value>;
     static unsigned long long ring_ok = 0;
     if (!allow_ring(kern, ring_ok)) return static_cast<int>(FRATTN_E_CUDA);
-    kern<<<norm_blocks(p.T, l, blocks), 32 * l.warps * l.teams, l.params + l.teams * l.team_bytes, st>>>(p, l);
-    return launched();
+    return launch_overlapped(kern, dim3(norm_blocks(p.T, l, blocks)), dim3(32 * l.warps * l.teams),
+                             l.params + l.teams * l.team_bytes, st, 1, p, l);
   });
 }
 
@@ -944,12 +956,11 @@ template <typename T, bool PACKED>
 int norm_bwd(const NormParams& p, int* groups, cudaStream_t st) {
   if (p.C > kMaxCols) {
     const int n = p.T < 2 * sms() ? p.T : 2 * sms();
-    layer_norm_bwd_wide_kernel<T, PACKED><<<n, 1024, 0, st>>>(p);
-    if (p.partial) {
-      *groups = p.T < sms() ? p.T : sms();
-      layer_norm_bwd_wide_cols_kernel<T, PACKED><<<dim3((p.C + 255) / 256, *groups), 256, 0, st>>>(p);
-    }
-    return launched();
+    const int rc = launch_overlapped(layer_norm_bwd_wide_kernel<T, PACKED>, dim3(n), dim3(1024), 0, st, 1, p);
+    if (rc || !p.partial) return rc;
+    *groups = p.T < sms() ? p.T : sms();
+    return launch_overlapped(layer_norm_bwd_wide_cols_kernel<T, PACKED>, dim3((p.C + 255) / 256, *groups), dim3(256), 0, st,
+                             1, p);
   }
   RowVec rv(p.C, sizeof(T));
   rv.row(p.x, p.x_stride).row(p.dy, p.dy_stride).row(p.out, p.out_stride);
@@ -964,8 +975,8 @@ int norm_bwd(const NormParams& p, int* groups, cudaStream_t st) {
     static unsigned long long ring_ok = 0;
     if (!allow_ring(kern, ring_ok)) return static_cast<int>(FRATTN_E_CUDA);
     *groups = norm_blocks(p.T, l, 1);
-    kern<<<*groups, 32 * l.warps * l.teams, l.params + l.teams * l.team_bytes, st>>>(p, l);
-    return launched();
+    return launch_overlapped(kern, dim3(*groups), dim3(32 * l.warps * l.teams), l.params + l.teams * l.team_bytes, st, 1,
+                             p, l);
   });
 }
 
@@ -995,10 +1006,9 @@ int pack(const PackParams& p, cudaStream_t st) {
   dim3 grid, block;
   const int nb = static_cast<int>(pack_blocks(p.C));
   pack_shape(nb * (kPackBlock / rv.v), p.T, &grid, &block);
-  if (rv.v == 8) act_pack_kernel<T, 8><<<grid, block, 0, st>>>(p);
-  else if (rv.v == 4) act_pack_kernel<T, 4><<<grid, block, 0, st>>>(p);
-  else act_pack_kernel<T, 1><<<grid, block, 0, st>>>(p);
-  return launched();
+  if (rv.v == 8) return launch_overlapped(act_pack_kernel<T, 8>, grid, block, 0, st, 1, p);
+  if (rv.v == 4) return launch_overlapped(act_pack_kernel<T, 4>, grid, block, 0, st, 1, p);
+  return launch_overlapped(act_pack_kernel<T, 1>, grid, block, 0, st, 1, p);
 }
 
 template <typename T>
@@ -1007,10 +1017,9 @@ int unpack(const PackParams& p, cudaStream_t st) {
   rv.row(p.out, p.out_stride);
   dim3 grid, block;
   pack_shape((p.C + rv.v - 1) / rv.v, p.T, &grid, &block);
-  if (rv.v == 8) act_unpack_kernel<T, 8><<<grid, block, 0, st>>>(p);
-  else if (rv.v == 4) act_unpack_kernel<T, 4><<<grid, block, 0, st>>>(p);
-  else act_unpack_kernel<T, 1><<<grid, block, 0, st>>>(p);
-  return launched();
+  if (rv.v == 8) return launch_overlapped(act_unpack_kernel<T, 8>, grid, block, 0, st, 1, p);
+  if (rv.v == 4) return launch_overlapped(act_unpack_kernel<T, 4>, grid, block, 0, st, 1, p);
+  return launch_overlapped(act_unpack_kernel<T, 1>, grid, block, 0, st, 1, p);
 }
 
 bool known_dtype(int d) { return d == FRATTN_F32 || d == FRATTN_F16 || d == FRATTN_BF16; }
@@ -1028,17 +1037,7 @@ int column_finish(const float* partial, int groups, int arrays, int C, void* out
   f.out[0] = out0;
   f.out[1] = out1;
   f.dtype = dtype;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3((C + 31) / 32, arrays);
-  lc.blockDim = dim3(32, 32);
-  lc.stream = st;
-  lc.attrs = &attr;
-  lc.numAttrs = 1;
-  if (cudaLaunchKernelEx(&lc, column_finish_kernel, f) != cudaSuccess) return FRATTN_E_CUDA;
-  return launched();
+  return launch_overlapped(column_finish_kernel, dim3((C + 31) / 32, arrays), dim3(32, 32), 0, st, 1, f);
 }
 
 // Checkpoint of a matrix back to 16-bit values (the linear layer's backward pass).
