@@ -19,6 +19,7 @@ from .fused_attn import (  # noqa: F401
     qkv_rope_projection,
     rope_positions_2d,
 )
+from .block import EncoderBlock  # noqa: F401
 from .block_ops import (  # noqa: F401
     ACTIVATIONS,
     PackedActivation,

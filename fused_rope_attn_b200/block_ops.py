@@ -96,16 +96,20 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t with rows that start on 16-byte boundaries (a TMA requirement): t itself, or a
-    copy in rows padded to a multiple of 8 elements. A weight whose width is not a
-    multiple of 8 is best kept that way by its owner (a ``[:, :K]`` view of a padded
-    buffer), so that no call copies it."""
+def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """t with rows that start on 16-byte boundaries (a TMA requirement), and their stride: t
+    itself, or a copy in rows padded to a multiple of 8 elements. A weight whose width is
+    not a multiple of 8 is best kept that way by its owner (a ``[:, :K]`` view of a
+    padded buffer), so that no call copies it."""
     n, k = t.shape
-    if ((t.stride(1) == 1 or k == 1) and t.data_ptr() % 16 == 0
-            and (n == 1 or t.stride(0) % 8 == 0 and t.stride(0) >= k)):
-        return t
-    return torch.empty(n, -(-k // 8) * 8, dtype=t.dtype, device=t.device)[:, :k].copy_(t)
+    s, c = t.stride()
+    if (c == 1 or k == 1) and t.data_ptr() % 16 == 0:
+        if n == 1:
+            return t, -(-k // 8) * 8
+        if s % 8 == 0 and s >= k:
+            return t, s
+    kp = -(-k // 8) * 8
+    return torch.empty(n, kp, dtype=t.dtype, device=t.device)[:, :k].copy_(t), kp
 
 
 def _stride(t: torch.Tensor) -> int:
@@ -200,7 +204,7 @@ def unpack_activation(p: PackedActivation, *, out: torch.Tensor | None = None) -
 def _check_param(name, t, C, dtype, device):
     if t.shape != (C,):
         raise ValueError(f"{name} must be [{C}], got {tuple(t.shape)}")
-    if t.dtype not in (dtype, torch.float32):
+    if t.dtype is not dtype and t.dtype is not torch.float32:
         raise ValueError(f"{name} dtype must be {dtype} or float32, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
@@ -231,15 +235,21 @@ def layer_norm(
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"weight and bias must share a dtype, got {weight.dtype} and {bias.dtype}")
     pd = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
-    x = _rows(x)
-    out = _check_out_rows(out, (T, C), x)
+    xs, xc = x.stride()
+    if xc != 1 and C > 1:
+        x, xs = x.contiguous(), C
     dev = x.device
+    if out is None:
+        out, os = torch.empty((T, C), dtype=x.dtype, device=dev), C
+    else:
+        out = _check_out_rows(out, (T, C), x)
+        os = _stride(out)
     mean = rstd = None
     if return_stats:
         mean = torch.empty(T, dtype=torch.float32, device=dev)
         rstd = torch.empty(T, dtype=torch.float32, device=dev)
-    _call("frattn_layer_norm", dev, x.data_ptr(), _stride(x), _ptr(weight), _ptr(bias), _DT[pd], T, C, eps,
-          _DT[x.dtype], out.data_ptr(), _stride(out), _ptr(mean), _ptr(rstd))
+    _call("frattn_layer_norm", dev, x.data_ptr(), xs, _ptr(weight), _ptr(bias), _DT[pd], T, C, eps,
+          _DT[x.dtype], out.data_ptr(), os, _ptr(mean), _ptr(rstd))
     return (out, mean, rstd) if return_stats else out
 
 
@@ -382,28 +392,27 @@ def linear_act(
         residual = _rows(residual)
     if save_preact not in (None, "none", "full", "packed"):
         raise ValueError(f"save_preact must be None, 'full' or 'packed', got {save_preact!r}")
-    out = _check_out_rows(out, (T, N), x)
+    if out is None:
+        out, out_stride = torch.empty((T, N), dtype=dt, device=dev), N
+    else:
+        out = _check_out_rows(out, (T, N), x)
+        out_stride = _stride(out)
     z = p = None
     if save_preact == "full":
         z = torch.empty(T, N, dtype=dt, device=dev)
     elif save_preact == "packed":
         p = _empty_packed(T, N, dt, dev)
     if T > 0:
-        x, weight = _rows16(x), _rows16(weight)
+        x, xs = _rows16(x)
+        weight, ws_ = _rows16(weight)
         nbytes = _workspace_bytes(_lib.workspace_bytes_linear_act, dev, T, K, N)
         ws = _workspace(nbytes, dev) if nbytes else None
-        _call("frattn_linear_act", dev, x.data_ptr(), _row16_stride(x), weight.data_ptr(), _row16_stride(weight),
-              _ptr(bias), _ptr(residual), 0 if residual is None else _stride(residual), act, T, K, N, _DT[dt],
-              out.data_ptr(), _stride(out), _ptr(z), N, p.codes.data_ptr() if p is not None else None,
+        _call("frattn_linear_act", dev, x.data_ptr(), xs, weight.data_ptr(), ws_, _ptr(bias), _ptr(residual),
+              0 if residual is None else _stride(residual), act, T, K, N, _DT[dt], out.data_ptr(), out_stride, _ptr(z), N, p.codes.data_ptr() if p is not None else None,
               p.scales.data_ptr() if p is not None else None, _ptr(ws), nbytes, _status_word(dev).data_ptr())
     if save_preact in (None, "none"):
         return out
     return out, (z if p is None else p)
-
-
-def _row16_stride(t: torch.Tensor) -> int:
-    """Row stride of a ``_rows16`` matrix (of a single row: any valid one)."""
-    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
 
 
 def linear_act_backward(
@@ -461,15 +470,16 @@ def linear_act_backward(
     db = torch.empty(N, dtype=dt, device=dev) if need_b else None
     if not (need_x or need_w or need_b):
         return dx, dw, db
-    if not xp and need_w:
-        x = _rows16(x)
+    xs, ws_ = K, K
+    if not xp:
+        x, xs = _rows16(x) if need_w else (x, max(_stride(x), K))
     if need_x:
-        weight = _rows16(weight)
+        weight, ws_ = _rows16(weight)
     nbytes = _workspace_bytes(_lib.workspace_bytes_linear_act_bwd, dev, T, K, N)
     ws = _workspace(nbytes, dev)
     _call("frattn_linear_act_bwd", dev, dout.data_ptr(), _stride(dout), None if xp else x.data_ptr(),
-          0 if xp else _row16_stride(x), x.codes.data_ptr() if xp else None, x.scales.data_ptr() if xp else None,
-          weight.data_ptr(), _row16_stride(weight), None if preact is None or zp else preact.data_ptr(),
+          0 if xp else xs, x.codes.data_ptr() if xp else None, x.scales.data_ptr() if xp else None,
+          weight.data_ptr(), ws_, None if preact is None or zp else preact.data_ptr(),
           0 if preact is None or zp else _stride(preact), preact.codes.data_ptr() if zp else None,
           preact.scales.data_ptr() if zp else None, act, T, K, N, _DT[dt], _ptr(dx), K, _ptr(dw), _ptr(db),
           ws.data_ptr(), nbytes, _status_word(dev).data_ptr())
@@ -483,7 +493,10 @@ class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, checkpoint):
         save = None if activation == "none" else "packed" if checkpoint else "full"
-        got = linear_act(x, weight, bias, activation=activation, residual=residual, save_preact=save)
+        T, N = x.shape[0], weight.shape[0]
+        # rows of whole 16 bytes, so that a following linear layer reads them in place
+        out = x.new_empty(T, -(-N // 8) * 8)[:, :N] if N % 8 and x.ndim == 2 else None
+        got = linear_act(x, weight, bias, activation=activation, residual=residual, out=out, save_preact=save)
         out, z = got if save else (got, None)
         ctx.activation, ctx.packed = activation, checkpoint
         ctx.has_bias, ctx.has_res = bias is not None, residual is not None
