@@ -940,10 +940,11 @@ struct ActBwdParams {
 };
 
 // One thread owns VEC columns over a strip of rows (rows blockIdx.y,
-// blockIdx.y + gridDim.y, ...): neighbouring threads read neighbouring vectors,
-// the column sums stay in registers, R rows are in flight at a time.
+// blockIdx.y + gridDim.y, ...): neighbouring threads read neighbouring vectors, the
+// column sums stay in registers, and the next R rows are on their way while R rows are
+// worked on.
 template <typename T, int VEC, int ACT, bool PACKED>
-__global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
+__global__ void __launch_bounds__(256, 2) act_bwd_kernel(const ActBwdParams p) {
   constexpr int R = 4;
   const int v = blockIdx.x * blockDim.x + threadIdx.x;
   griddep_wait();
@@ -955,25 +956,44 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
 #pragma unroll
   for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
   const long long step = gridDim.y;
+  Vec<T, VEC> ndy[R], nz[R];
+  CodeVec<VEC> nq[R];
+  uint32_t nscale[R];
+  auto fetch = [&](long long row0) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = row0 + r * step;
+      if (row < p.T) {
+        ndy[r].load(static_cast<const T*>(p.dout) + row * p.dout_stride + c);
+        if constexpr (ACT != FRATTN_ACT_NONE) {
+          if constexpr (PACKED) {
+            nq[r].load(p.z_codes + row * nb * kPackBlock + c);
+            nscale[r] = __ldcg(p.z_scales + row * nb + v * VEC / kPackBlock);
+          } else {
+            nz[r].load(static_cast<const T*>(p.z) + row * p.z_stride + c);
+          }
+        }
+      }
+    }
+  };
+  fetch(blockIdx.y);
   for (long long row0 = blockIdx.y; row0 < p.T; row0 += step * R) {
     Vec<T, VEC> dy[R], z[R];
     CodeVec<VEC> q[R];
     uint32_t scale[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long long row = row0 + r * step;
-      if (row < p.T) {
-        dy[r].load(static_cast<const T*>(p.dout) + row * p.dout_stride + c);
-        if constexpr (ACT != FRATTN_ACT_NONE) {
-          if constexpr (PACKED) {
-            q[r].load(p.z_codes + row * nb * kPackBlock + c);
-            scale[r] = __ldcg(p.z_scales + row * nb + v * VEC / kPackBlock);
-          } else {
-            z[r].load(static_cast<const T*>(p.z) + row * p.z_stride + c);
-          }
+      dy[r] = ndy[r];
+      if constexpr (ACT != FRATTN_ACT_NONE) {
+        if constexpr (PACKED) {
+          q[r] = nq[r];
+          scale[r] = nscale[r];
+        } else {
+          z[r] = nz[r];
         }
       }
     }
+    fetch(row0 + step * R);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + r * step;
@@ -985,13 +1005,11 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
         if constexpr (PACKED) q[r].get(pack_step(scale[r]), f);
         else z[r].get(f);
 #pragma unroll
-        for (int e = 0; e + 1 < VEC; e += 2) act_grad_f2<ACT>(f[e], f[e + 1]);
+        for (int e = 0; e + 1 < VEC; e += 2) act_grad_f2<ACT>(f[e], f[e + 1], d[e], d[e + 1]);
         if constexpr (VEC == 1) {
           float none = 0.f;
-          act_grad_f2<ACT>(f[0], none);
+          act_grad_f2<ACT>(f[0], 0.f, d[0], none);
         }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) d[e] *= f[e];
       }
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sum[e] += d[e];

@@ -750,9 +750,9 @@ struct PackParams {
 // One vector of VEC columns per thread and row, 32 / VEC neighbouring threads per
 // block of 32 values. Columns past C (the last block of a row) are zeros.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) act_pack_kernel(const PackParams p) {
+__global__ void __launch_bounds__(256, 8) act_pack_kernel(const PackParams p) {
   constexpr int G = kPackBlock / VEC;  // threads of a block of 32
-  constexpr int R = 4;
+  constexpr int R = 1;  // (the warps of a full SM keep enough on its way; 4 rows to a thread took half as long again)
   const int nb = static_cast<int>(pack_blocks(p.C));
   const int v = blockIdx.x * blockDim.x + threadIdx.x;
   griddep_wait();
@@ -771,27 +771,30 @@ __global__ void __launch_bounds__(256) act_pack_kernel(const PackParams p) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + r * step;
-      uint32_t m = 0;
       float f[VEC];
       x[r].get(f);
+      if (!has) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (!has) f[e] = 0.f;
-        m = max(m, abs_bits(f[e]));
+        for (int e = 0; e < VEC; ++e) f[e] = 0.f;
       }
+      float m = 0.f;
 #pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const uint32_t scale = pack_scale(m);
-      const float inv = pack_inv(scale), lim = pack_limit(scale);
+      for (int e = 0; e + 1 < VEC; e += 2) m = max3_abs(m, f[e], f[e + 1]);
+      if constexpr (VEC == 1) m = fabsf(f[0]);
+      uint32_t amax = abs_bits(m);  // (as integers a NaN is the largest)
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      const uint32_t scale = pack_scale(amax);
       if (in_row && row < p.T) {
         int8_t* dst = p.codes + row * nb * kPackBlock + static_cast<size_t>(v) * VEC;
+        const float inv = pack_inv(scale);
         if constexpr (VEC == 1) {
-          *dst = static_cast<int8_t>(pack_code(f[0], inv, lim));
-        } else if constexpr (VEC == 4) {
-          *reinterpret_cast<uint32_t*>(dst) = pack_code4(f[0], f[1], f[2], f[3], inv, lim);
+          *dst = static_cast<int8_t>(pack_code(f[0], inv, pack_limit(scale)));
         } else {
-          *reinterpret_cast<uint2*>(dst) = make_uint2(pack_code4(f[0], f[1], f[2], f[3], inv, lim),
-                                                      pack_code4(f[4], f[5], f[6], f[7], inv, lim));
+          uint32_t codes[VEC / 4];
+          pack_codes<VEC>(f, __uint_as_float(amax), scale, codes);
+          if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(dst) = codes[0];
+          else *reinterpret_cast<uint2*>(dst) = make_uint2(codes[0], codes[1]);
         }
         if (v % G == 0) p.scales[row * nb + v / G] = static_cast<uint8_t>(scale);
       }

@@ -500,3 +500,33 @@ def test_gradients_of_broadcast_outputs():
     nx = x.to(DEV).requires_grad_(True)
     fr.layer_norm_train(nx).sum().backward()
     assert nx.grad.abs().max() <= 2.0 ** -6  # the sum of a row's outputs is constant
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_activations_over_their_whole_range(act, dt):
+    """Every magnitude the type has, forward (K = 1, weight 1: z = x) and derivative: near the
+    formula within the approximations' 2^-20 of |z| (1 + |z|) for the derivative's factor, and a
+    NaN or an infinity changes no other column."""
+    mag = torch.logspace(-6, 4.5, 400, dtype=torch.float64)
+    z = torch.cat([mag, -mag, torch.zeros(1, dtype=torch.float64)]).to(dt)
+    z = z[torch.isfinite(z)]
+    N = z.numel()
+    x = torch.ones(1, 1, dtype=dt, device=DEV)
+    y = fr.linear_act(x, z.view(N, 1).to(DEV), activation=act)
+    zz = f64(z)
+    with np.errstate(over="ignore", invalid="ignore"):
+        ry, rg = B.act(zz, act), B.act_grad(np.clip(zz, -1e3, 1e3), act)
+    near(y[0], ry, dt, 2.0 ** -20 * np.abs(zz))
+    eye = torch.eye(1, dtype=dt, device=DEV)
+    _, _, db = fr.linear_act_backward(torch.ones(1, N, dtype=dt, device=DEV), eye, z.view(N, 1).to(DEV), z.view(1, N).to(DEV),
+                                      activation=act)
+    near(db, rg, dt, 2.0 ** -20 * (1 + np.minimum(np.abs(zz), 64)))
+    bad = z.clone()
+    bad[7], bad[100] = float("nan"), float("inf")
+    keep = [i for i in range(N) if i not in (7, 100)]
+    yb = fr.linear_act(x, bad.view(N, 1).to(DEV), activation=act)
+    assert torch.equal(yb[0][keep], y[0][keep]) and torch.isnan(yb[0, 7]) and yb[0, 100] == float("inf")
+    _, _, gb = fr.linear_act_backward(torch.ones(1, N, dtype=dt, device=DEV), eye, z.view(N, 1).to(DEV), bad.view(1, N).to(DEV),
+                                      activation=act)
+    assert torch.equal(gb[keep], db[keep]) and torch.isnan(gb[7]) and gb[100] == 1
