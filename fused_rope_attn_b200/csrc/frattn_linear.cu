@@ -30,9 +30,10 @@ struct GemmParams {
   long long z_stride;
   int8_t* z_codes;  // or null
   uint8_t* z_scales;
-  int out_tma, z_tma;          // written by TMA stores (16-byte rows), else by element stores of
-  int out_w, z_w;              // 4, 2 or 1 elements
+  int out_tma, z_tma;          // written by TMA stores (16-byte rows; the pair kernel)
+  int out_w, z_w;              // else elements per store: 8 (where N allows it), 4, 2 or 1
   int res_tma;                 // residual read ahead by TMA (16-byte rows, nothing else staged)
+  int res_vec;                 // residual rows are 16-byte aligned
   int M, N, nk;                // nk: 64-wide steps of the reduction
   int a_bytes;                 // of A in a stage (small products)
   int tiles_n, tiles;
@@ -199,7 +200,7 @@ __device__ __forceinline__ void store_staged(const CUtensorMap* map, int tma, in
     }
   } else {
     __syncwarp();
-    if (width == 4) store_rows_w<4>(stg, lane, out, stride, m0, n0, M, N);
+    if (width >= 4) store_rows_w<4>(stg, lane, out, stride, m0, n0, M, N);
     else if (width == 2) store_rows_w<2>(stg, lane, out, stride, m0, n0, M, N);
     else store_rows_w<1>(stg, lane, out, stride, m0, n0, M, N);
     __syncwarp();
@@ -222,31 +223,48 @@ __device__ __forceinline__ void add_bias(float (&v)[32], const float* bias) {
   }
 }
 
-// The epilogue of 32 columns [n, n + 32) of a row by one thread, straight to memory (the
-// joined parts of a split product; columns past N hold zeros).
-template <typename T>
-__device__ __forceinline__ void put32(void* base, long long stride, long long row, int n, int N, int width, const float (&v)[32]) {
-  T* dst = static_cast<T*>(base) + row * stride + n;
-  if (width == 8 && n + 32 <= N) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      reinterpret_cast<uint4*>(dst)[c] = make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
-                                                    pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (n + i < N) dst[i] = f32_elem<T>(v[i]);
+// The epilogue of a warp's piece of D, rows [m, m + 32) (one a lane) and columns
+// [n, n + 32), of which v holds the lane's row (columns past N hold zeros). `stg`: 2 KB of
+// the warp's own, through which rows are written a row's parts in neighbouring lanes
+// (16-byte part c of row r at c ^ (r / 2 & 3), 64-byte rows).
+template <typename T, int W>
+__device__ __forceinline__ void put_piece_w(const uint8_t* stg, int lane, void* out, long long stride, long long m, int n,
+                                            int M, int N) {
+  using Raw = typename RawVec<2 * W>::type;
+  constexpr int LANES = 32 / W;  // lanes of a row
+#pragma unroll 8
+  for (int i = lane; i < 32 * LANES; i += 32) {
+    const int r = i / LANES, c = i % LANES * W;
+    if (m + r < M && n + c < N)  // (W divides N: a vector lies inside the row or outside)
+      *reinterpret_cast<Raw*>(static_cast<uint16_t*>(out) + (m + r) * stride + n + c) =
+          *reinterpret_cast<const Raw*>(stg + r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) << 4) + (c & 7) * 2);
   }
 }
 template <typename T>
-__device__ __forceinline__ void finish_row(const GemmParams& p, long long row, int n, float (&v)[32]) {
-  if (p.bias) {
+__device__ __forceinline__ void put_piece(uint8_t* stg, int lane, void* out, long long stride, long long m, int n, int M,
+                                          int N, int width, const float (&v)[32]) {
+  __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (n + i < p.N) v[i] += elem_f32<T>(static_cast<const T*>(p.bias)[n + i]);
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<uint4*>(stg + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
+                   pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
+  __syncwarp();
+  if (width == 8) put_piece_w<T, 8>(stg, lane, out, stride, m, n, M, N);
+  else if (width == 4) put_piece_w<T, 4>(stg, lane, out, stride, m, n, M, N);
+  else if (width == 2) put_piece_w<T, 2>(stg, lane, out, stride, m, n, M, N);
+  else put_piece_w<T, 1>(stg, lane, out, stride, m, n, M, N);
+}
+template <typename T>
+__device__ __forceinline__ void finish_piece(const GemmParams& p, long long m, int n, int lane, uint8_t* stg, float (&v)[32]) {
+  const long long row = m + lane;
+  if (p.bias) {
+    const float b = n + lane < p.N ? elem_f32<T>(static_cast<const T*>(p.bias)[n + lane]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, b, i);
   }
-  if (p.z) put32<T>(p.z, p.z_stride, row, n, p.N, p.z_tma ? 8 : 1, v);
-  if (p.z_codes) {
+  if (p.z) put_piece<T>(stg, lane, p.z, p.z_stride, m, n, p.M, p.N, p.z_w, v);
+  if (p.z_codes && row < p.M) {
     const long long nb = pack_blocks(p.N);
     uint32_t codes[8];
     p.z_scales[row * nb + n / 32] = static_cast<uint8_t>(pack32(v, codes));
@@ -256,13 +274,23 @@ __device__ __forceinline__ void finish_row(const GemmParams& p, long long row, i
           make_uint4(codes[4 * c], codes[4 * c + 1], codes[4 * c + 2], codes[4 * c + 3]);
   }
   act_any(p.act, v);
-  if (p.res) {
+  if (p.res && row < p.M) {
     const T* rp = static_cast<const T*>(p.res) + row * p.res_stride + n;
+    if (p.res_vec && n + 32 <= p.N) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (n + i < p.N) v[i] += elem_f32<T>(rp[i]);
+      for (int c = 0; c < 4; ++c) {
+        float f[8];
+        unpack8<T>(reinterpret_cast<const uint4*>(rp)[c], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * c + e] += f[e];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (n + i < p.N) v[i] += elem_f32<T>(rp[i]);
+    }
   }
-  put32<T>(p.out, p.out_stride, row, n, p.N, p.out_tma ? 8 : 1, v);
+  put_piece<T>(stg, lane, p.out, p.out_stride, m, n, p.M, p.N, p.out_w, v);
 }
 
 // GEMM on CTA pairs (cluster of 2, tcgen05 cta_group::2): 256 x BN tiles of D, M = 256
@@ -547,30 +575,35 @@ __global__ void __launch_bounds__(256) gemm_finish_kernel(const __grid_constant_
     griddep_wait();
     return;
   }
-  const int unit = blockIdx.y * 8 + static_cast<int>(threadIdx.x >> 5);  // of 32 rows x 32 columns
-  const int r = unit % 8 * 32 + static_cast<int>(threadIdx.x & 31), c = unit / 8 * 32;
-  const long long row = static_cast<long long>(t / p.tiles_n) * 256 + r;
+  __shared__ __align__(16) uint8_t stage[8][2048];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int unit = blockIdx.y * 8 + warp;  // of 32 rows x 32 columns
+  const int r = unit % 8 * 32 + lane, c = unit / 8 * 32;
+  const long long m = static_cast<long long>(t / p.tiles_n) * 256 + unit % 8 * 32;
   const int n = (t % p.tiles_n) * BN + c;
   griddep_wait();
   griddep_launch_dependents();
-  if (row >= p.M || n >= p.N) return;
+  if (m >= p.M || n >= p.N) return;
   float v[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = 0.f;
-  for (int q = first; q <= last; ++q) {
-    const long long b = static_cast<long long>(q) * p.split;
-    const int slot = 2 * q + (b > static_cast<long long>(t) * p.nk ? 0 : 1);  // began inside the tile, or before or at its first step
-    const float4* src = reinterpret_cast<const float4*>(p.partial) + (static_cast<size_t>(slot) * (BN / 4) + c / 4) * 256 + r;
+  if (m + lane < p.M) {
+    for (int q = first; q <= last; ++q) {
+      const long long b = static_cast<long long>(q) * p.split;
+      const int slot = 2 * q + (b > static_cast<long long>(t) * p.nk ? 0 : 1);  // began inside the tile, or before or at its first step
+      const float4* src = reinterpret_cast<const float4*>(p.partial) + (static_cast<size_t>(slot) * (BN / 4) + c / 4) * 256 + r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 x = __ldcg(src + i * 256);
-      v[4 * i] += x.x;
-      v[4 * i + 1] += x.y;
-      v[4 * i + 2] += x.z;
-      v[4 * i + 3] += x.w;
+      for (int i = 0; i < 8; ++i) {
+        const float4 x = __ldcg(src + i * 256);
+        v[4 * i] += x.x;
+        v[4 * i + 1] += x.y;
+        v[4 * i + 2] += x.z;
+        v[4 * i + 3] += x.w;
+      }
     }
   }
-  finish_row<T>(p, row, n, v);
+  __syncwarp();
+  finish_piece<T>(p, m, n, lane, stage[warp], v);
 }
 
 // ------------------------------------------------------------------ small products
@@ -588,7 +621,7 @@ struct SmallCfg {
   static constexpr int OFF_BAR = ST * STAGE;
   static constexpr int SMEM = OFF_BAR + 128 + 1024;
   static constexpr int THREADS = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
-  static_assert(SUM_BYTES <= ST * STAGE, "sums fit");
+  static_assert(SUM_BYTES + 4 * 2048 <= ST * STAGE, "sums and the warps' staging fit");
 };
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
@@ -678,13 +711,13 @@ __global__ void __launch_bounds__(SmallCfg::THREADS) gemm_small_kernel(const __g
   __syncwarp();
   const int quarter = warp & 3;
   const bool rows = warp >= 2 && m0 + quarter * 32 < p.M;  // an epilogue warp with rows of D
-  const long long row = m0 + quarter * 32 + lane;
   bool ok = true;
   if (rows) {
     ok = __all_sync(0xffffffffu, gemm_wait(bar(ACC), 0, p, abort_flag, FRATTN_STATUS_WAIT_TIMEOUT | 0x78));
     tc_fence_after();
   }
   const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  uint8_t* stg = smem + C::SUM_BYTES + quarter * 2048;  // (free once all MMAs are done)
   if (S == 1) {
     if (rows && ok) {
 #pragma unroll 1
@@ -693,7 +726,7 @@ __global__ void __launch_bounds__(SmallCfg::THREADS) gemm_small_kernel(const __g
         float v[32];
         tmem_ld32(acc + 32 * h, reinterpret_cast<uint32_t (&)[32]>(v));
         tmem_ld_wait();
-        if (row < p.M) finish_row<T>(p, row, n0 + 32 * h, v);
+        finish_piece<T>(p, m0 + quarter * 32, n0 + 32 * h, lane, stg, v);
       }
     }
   } else {
@@ -713,25 +746,28 @@ __global__ void __launch_bounds__(SmallCfg::THREADS) gemm_small_kernel(const __g
     cluster_sync_all();  // every CTA's sums are written (a CTA without rows or timed out has none to read)
     // this CTA's share of the tile's (row, 32 columns) units
     if (warp >= 2) {
-      const int share = 256 / S, t = (warp - 2) * 32 + lane;
-      for (int u = rank * share + t; u < (rank + 1) * share; u += 128) {
+      const int share = 256 / S;  // 32 rows a warp at a time: a multiple of 32
+      for (int u = rank * share + (warp - 2) * 32; u < (rank + 1) * share; u += 128) {
         const int r = u & 127, h = u >> 7, n = n0 + 32 * h;
         if (m0 + r >= p.M || n >= p.N) continue;
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = 0.f;
-        for (int q = 0; q < S; ++q) {
-          const uint32_t from = mapa_shared(smem_u32(sums + (8 * h) * 128 + r), q);
+        if (m0 + r + lane < p.M) {
+          for (int q = 0; q < S; ++q) {
+            const uint32_t from = mapa_shared(smem_u32(sums + (8 * h) * 128 + r + lane), q);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const float4 x = ld_cluster_f4(from + c * 128 * 16);
-            v[4 * c] += x.x;
-            v[4 * c + 1] += x.y;
-            v[4 * c + 2] += x.z;
-            v[4 * c + 3] += x.w;
+            for (int c = 0; c < 8; ++c) {
+              const float4 x = ld_cluster_f4(from + c * 128 * 16);
+              v[4 * c] += x.x;
+              v[4 * c + 1] += x.y;
+              v[4 * c + 2] += x.z;
+              v[4 * c + 3] += x.w;
+            }
           }
         }
-        finish_row<T>(p, m0 + r, n, v);
+        __syncwarp();
+        finish_piece<T>(p, m0 + r, n, lane, stg, v);
       }
     }
     cluster_sync_all();  // nobody leaves while its sums may be read
@@ -903,7 +939,7 @@ int gemm(GemmParams& p, const Mat& a, const Mat& b, int M, int N, int K, void* w
       encode_map(&p.tma_b, b.p, BMN ? N : K, BMN ? K : N, b.stride, 64, BMN || small ? 64 : plan.bn / 2, bf16))
     return FRATTN_E_TMAP;
   auto width = [&](const void* q, long long stride) {
-    for (int w = 4; w > 1; w >>= 1)
+    for (int w = 8; w > 1; w >>= 1)
       if (aligned_to(q, 2 * w) && stride % w == 0 && N % w == 0) return w;
     return 1;
   };
@@ -916,6 +952,7 @@ int gemm(GemmParams& p, const Mat& a, const Mat& b, int M, int N, int K, void* w
     if (p.z_tma && !small && encode_map(&p.tma_z, p.z, N, M, p.z_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
   }
   if (p.z_codes && !small && encode_codes_map(&p.tma_codes, p.z_codes, pack_blocks(N) * kPackBlock, M)) return FRATTN_E_TMAP;
+  p.res_vec = p.res && rows16(p.res, p.res_stride);
   if (small) return gemm_small_launch<AMN, BMN, T>(p, plan, st);
   p.res_tma = p.res && rows16(p.res, p.res_stride) && p.res_stride >= N && !p.z && !p.z_codes;
   if (p.res_tma && encode_map(&p.tma_res, p.res, N, M, p.res_stride, 64, 32, bf16)) return FRATTN_E_TMAP;
