@@ -80,12 +80,15 @@ struct Vec {
   static __device__ __forceinline__ void put(T* p, const float (&v)[VEC]) {
     if constexpr (std::is_same<T, float>::value) {
       if constexpr (VEC == 1) p[0] = v[0];
+      else if constexpr (VEC == 2) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
       else
 #pragma unroll
         for (int i = 0; i < VEC / 4; ++i)
           reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
     } else if constexpr (VEC == 1) {
       p[0] = f32_elem<T>(v[0]);
+    } else if constexpr (VEC == 2) {
+      *reinterpret_cast<uint32_t*>(p) = pack2<T>(v[0], v[1]);
     } else if constexpr (VEC == 4) {
       *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
     } else {
@@ -109,13 +112,13 @@ struct CodeVec {
   }
 };
 
-// Largest vector width of {8, 4, 1} elements of esz bytes that every listed
+// Largest vector width of {8, 4, 2, 1} elements of esz bytes that every listed
 // pointer and row stride (elements) allows for rows of C elements.
 struct RowVec {
   int C, esz;
   int v = 8;
   RowVec(int C_, int esz_) : C(C_), esz(esz_) {
-    while (v > 1 && C % v) v = v == 8 ? 4 : 1;
+    while (C % v) v /= 2;
   }
   RowVec& row(const void* p, long long stride, int e = 0) {
     if (!p) return *this;
@@ -124,7 +127,7 @@ struct RowVec {
       const int a = w * es < 16 ? w * es : 16;
       return reinterpret_cast<uintptr_t>(p) % a == 0 && (stride * es) % a == 0;
     };
-    while (v > 1 && !ok(v)) v = v == 8 ? 4 : 1;
+    while (v > 1 && !ok(v)) v /= 2;
     return *this;
   }
 };

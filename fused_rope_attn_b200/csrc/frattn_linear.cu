@@ -841,11 +841,13 @@ GemmPlan gemm_plan(int M, int N, int nk) {
   const int P = sm_pairs();
   double best_us = 1e30;
   {
-    // 128 x 64 tiles, up to 8 CTAs on one while that leaves each two steps and two CTAs to
-    // an SM: bound by 24 KB from L2 a step (10 TB/s for all), or by latency
+    // 128 x 64 tiles, up to 8 CTAs on one while that leaves each two steps, and all of them
+    // run at once: two fit an SM, but clusters of 8 have to fit its processing cluster
+    // too, so that 37 clusters of 8 took two rounds (21 us; 10 with 4). Bound by 24 KB
+    // from L2 a step (10 TB/s for all), or by latency.
     const long long tiles = static_cast<long long>((M + 127) / 128) * ((N + 63) / 64);
     int S = 1;
-    while (S < 8 && tiles * 2 * S <= 4 * P && nk >= 4 * S) S *= 2;
+    while (S < 8 && tiles * 2 * S <= 3 * P && nk >= 4 * S) S *= 2;
     const double rows = M < 128 ? M : 128;
     const double us = tiles * nk * (rows * 128 + 8192) / 10e6 + 0.25 * ((nk + S - 1) / S) * ((tiles * S + 4 * P - 1) / (4 * P)) + 1.0;
     if (tiles * S < (1 << 30)) {
@@ -1096,6 +1098,7 @@ int act_bwd(const ActBwdParams& p, int act, int* groups, cudaStream_t st) {
   rv.row(p.dout, p.dout_stride).row(p.z, p.z_stride).row(p.dz, p.dz_stride);
   if (rv.v == 8) return p.z_codes ? act_bwd_act<T, 8, true>(p, act, groups, st) : act_bwd_act<T, 8, false>(p, act, groups, st);
   if (rv.v == 4) return p.z_codes ? act_bwd_act<T, 4, true>(p, act, groups, st) : act_bwd_act<T, 4, false>(p, act, groups, st);
+  if (rv.v == 2) return p.z_codes ? act_bwd_act<T, 2, true>(p, act, groups, st) : act_bwd_act<T, 2, false>(p, act, groups, st);
   return p.z_codes ? act_bwd_act<T, 1, true>(p, act, groups, st) : act_bwd_act<T, 1, false>(p, act, groups, st);
 }
 

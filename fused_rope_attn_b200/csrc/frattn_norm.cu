@@ -790,6 +790,10 @@ __global__ void __launch_bounds__(256, 8) act_pack_kernel(const PackParams p) {
         const float inv = pack_inv(scale);
         if constexpr (VEC == 1) {
           *dst = static_cast<int8_t>(pack_code(f[0], inv, pack_limit(scale)));
+        } else if constexpr (VEC == 2) {
+          const float lim = pack_limit(scale);
+          *reinterpret_cast<uint16_t*>(dst) =
+              static_cast<uint16_t>(__byte_perm(pack_code(f[0], inv, lim), pack_code(f[1], inv, lim), 0x0040));
         } else {
           uint32_t codes[VEC / 4];
           pack_codes<VEC>(f, __uint_as_float(amax), scale, codes);
@@ -934,6 +938,7 @@ int norm_fwd(NormParams p, cudaStream_t st) {
   }
   RowVec rv(p.C, sizeof(T));
   rv.row(p.x, p.x_stride).row(p.out, p.out_stride);
+  if (rv.v == 2) rv.v = 1;
   if (p.T <= kFewRows * sms()) {
     p.w_vec = aligned_to(p.w, 16) && aligned_to(p.b, 16);
     const int warps = short_team_warps(p.C);
@@ -967,6 +972,7 @@ int norm_bwd(const NormParams& p, int* groups, cudaStream_t st) {
   }
   RowVec rv(p.C, sizeof(T));
   rv.row(p.x, p.x_stride).row(p.dy, p.dy_stride).row(p.out, p.out_stride);
+  if (rv.v == 2) rv.v = 1;
   const int warps = p.T <= kFewRows * sms() ? short_team_warps(p.C) : bwd_team_warps(p.C, rv.v, PACKED);
   const int gradients = 2 * p.C * 4;  // a team's, in the end
   const NormLayout l = norm_layout(p.T, p.C, warps, 384, 1, 1, gradients, [](int cols) {
@@ -1011,6 +1017,7 @@ int pack(const PackParams& p, cudaStream_t st) {
   pack_shape(nb * (kPackBlock / rv.v), p.T, &grid, &block);
   if (rv.v == 8) return launch_overlapped(act_pack_kernel<T, 8>, grid, block, 0, st, 1, p);
   if (rv.v == 4) return launch_overlapped(act_pack_kernel<T, 4>, grid, block, 0, st, 1, p);
+  if (rv.v == 2) return launch_overlapped(act_pack_kernel<T, 2>, grid, block, 0, st, 1, p);
   return launch_overlapped(act_pack_kernel<T, 1>, grid, block, 0, st, 1, p);
 }
 
@@ -1022,6 +1029,7 @@ int unpack(const PackParams& p, cudaStream_t st) {
   pack_shape((p.C + rv.v - 1) / rv.v, p.T, &grid, &block);
   if (rv.v == 8) return launch_overlapped(act_unpack_kernel<T, 8>, grid, block, 0, st, 1, p);
   if (rv.v == 4) return launch_overlapped(act_unpack_kernel<T, 4>, grid, block, 0, st, 1, p);
+  if (rv.v == 2) return launch_overlapped(act_unpack_kernel<T, 2>, grid, block, 0, st, 1, p);
   return launch_overlapped(act_unpack_kernel<T, 1>, grid, block, 0, st, 1, p);
 }
 
