@@ -46,18 +46,21 @@ PACK_BLOCK = 32
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_entries: dict = {}
+# The current stream's handle and device alone, where torch has them: the public calls
+# build objects around them, a quarter of a small call's time.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _call(name: str, device: torch.device, *args) -> None:
     """Calls a C entry on ``device`` with its current stream as the last argument."""
-    fn = getattr(_lib.load(), name)
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
     i = device.index
-    if i is None or i == torch.cuda.current_device():
-        # the handle alone: torch.cuda.current_stream builds an object around it, 2 us of a
-        # small call's 10
-        stream = _raw_stream(i) if _raw_stream and i is not None else torch.cuda.current_stream(device).cuda_stream
-        rc = fn(*args, stream)
+    if i is not None and i == _current_device():
+        rc = fn(*args, _raw_stream(i) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream)
     else:
         with torch.cuda.device(device):
             rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
@@ -149,21 +152,22 @@ class PackedActivation(NamedTuple):
 
 
 def _check_packed(name, p, dtype=None, shape=None):
-    t, nb = p.scales.shape if p.scales.ndim == 2 else (-1, -1)
-    if nb != -(-p.width // PACK_BLOCK) or p.width <= 0 or tuple(p.codes.shape) != (t, nb * PACK_BLOCK):
-        raise ValueError(f"{name}: codes {tuple(p.codes.shape)} and scales {tuple(p.scales.shape)} do not hold "
-                         f"rows of {p.width} values in blocks of {PACK_BLOCK}")
-    if p.codes.dtype != torch.int8 or p.scales.dtype != torch.uint8 or p.codes.device != p.scales.device:
-        raise ValueError(f"{name}: codes must be int8 and scales uint8 on one device, got {p.codes.dtype} on "
-                         f"{p.codes.device} and {p.scales.dtype} on {p.scales.device}")
-    if p.codes.device.type != "cuda":
-        raise ValueError(f"{name} must be on CUDA, got device={p.codes.device}")
-    if not p.codes.is_contiguous() or not p.scales.is_contiguous() or p.codes.data_ptr() % 16:
+    codes, scales, width, dt = p
+    t, nb = scales.shape if scales.ndim == 2 else (-1, -1)
+    if nb != -(-width // PACK_BLOCK) or width <= 0 or codes.shape != (t, nb * PACK_BLOCK):
+        raise ValueError(f"{name}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold "
+                         f"rows of {width} values in blocks of {PACK_BLOCK}")
+    if codes.dtype is not torch.int8 or scales.dtype is not torch.uint8 or codes.device != scales.device:
+        raise ValueError(f"{name}: codes must be int8 and scales uint8 on one device, got {codes.dtype} on "
+                         f"{codes.device} and {scales.dtype} on {scales.device}")
+    if not codes.is_cuda:
+        raise ValueError(f"{name} must be on CUDA, got device={codes.device}")
+    if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16:
         raise ValueError(f"{name}: codes and scales must be contiguous, codes 16-byte aligned")
-    if shape is not None and tuple(p.shape) != tuple(shape):
-        raise ValueError(f"{name} must stand for {tuple(shape)}, got {tuple(p.shape)}")
-    if dtype is not None and p.dtype != dtype:
-        raise ValueError(f"{name} must stand for {dtype}, got {p.dtype}")
+    if shape is not None and (t, width) != tuple(shape):
+        raise ValueError(f"{name} must stand for {tuple(shape)}, got {(t, width)}")
+    if dtype is not None and dt != dtype:
+        raise ValueError(f"{name} must stand for {dtype}, got {dt}")
 
 
 def _empty_packed(rows, width, dtype, device) -> PackedActivation:
@@ -179,10 +183,13 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
     ``2**max(q - 7, -126)`` and each value is rounded to the nearest multiple of it
     (ties to even; at most 127 steps)."""
     _check_rows("x", x, tuple(_DT))
-    x = _rows(x)
-    p = _empty_packed(x.shape[0], x.shape[1], x.dtype, x.device)
-    _call("frattn_act_pack", x.device, x.data_ptr(), _stride(x), x.shape[0], x.shape[1], _DT[x.dtype],
-          p.codes.data_ptr(), p.scales.data_ptr())
+    T, C = x.shape
+    dt, dev = x.dtype, x.device
+    xs, xc = x.stride()
+    if xc != 1 and C > 1:
+        x, xs = x.contiguous(), C
+    p = _empty_packed(T, C, dt, dev)
+    _call("frattn_act_pack", dev, x.data_ptr(), xs, T, C, _DT[dt], p.codes.data_ptr(), p.scales.data_ptr())
     return p
 
 
@@ -191,12 +198,14 @@ def unpack_activation(p: PackedActivation, *, out: torch.Tensor | None = None) -
     _check_packed("packed activation", p)
     if p.dtype not in _DT:
         raise ValueError(f"dtype must be float16, bfloat16 or float32, got {p.dtype}")
+    codes, scales, C, dt = p
+    T, dev = scales.shape[0], codes.device
     if out is None:
-        out = torch.empty(p.shape, dtype=p.dtype, device=p.device)
+        out, os = torch.empty((T, C), dtype=dt, device=dev), C
     else:
-        out = _check_out_rows(out, p.shape, torch.empty(0, dtype=p.dtype, device=p.device))
-    _call("frattn_act_unpack", p.device, p.codes.data_ptr(), p.scales.data_ptr(), p.shape[0], p.width,
-          _DT[p.dtype], out.data_ptr(), _stride(out))
+        out = _check_out_rows(out, (T, C), torch.empty(0, dtype=dt, device=dev))
+        os = _stride(out)
+    _call("frattn_act_unpack", dev, codes.data_ptr(), scales.data_ptr(), T, C, _DT[dt], out.data_ptr(), os)
     return out
 
 
@@ -230,27 +239,32 @@ def layer_norm(
     T, C = x.shape
     if not eps >= 0:
         raise ValueError(f"eps must be >= 0, got {eps}")
-    weight = None if weight is None else _check_param("weight", weight, C, x.dtype, x.device)
-    bias = None if bias is None else _check_param("bias", bias, C, x.dtype, x.device)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError(f"weight and bias must share a dtype, got {weight.dtype} and {bias.dtype}")
-    pd = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+    dt, dev = x.dtype, x.device
+    pd, wp, bp = dt, None, None
+    if weight is not None:
+        weight = _check_param("weight", weight, C, dt, dev)
+        pd, wp = weight.dtype, weight.data_ptr()
+    if bias is not None:
+        bias = _check_param("bias", bias, C, dt, dev)
+        if weight is not None and bias.dtype is not pd:
+            raise ValueError(f"weight and bias must share a dtype, got {pd} and {bias.dtype}")
+        pd, bp = bias.dtype, bias.data_ptr()
     xs, xc = x.stride()
     if xc != 1 and C > 1:
         x, xs = x.contiguous(), C
-    dev = x.device
     if out is None:
-        out, os = torch.empty((T, C), dtype=x.dtype, device=dev), C
+        out, os = torch.empty((T, C), dtype=dt, device=dev), C
     else:
         out = _check_out_rows(out, (T, C), x)
         os = _stride(out)
-    mean = rstd = None
-    if return_stats:
-        mean = torch.empty(T, dtype=torch.float32, device=dev)
-        rstd = torch.empty(T, dtype=torch.float32, device=dev)
-    _call("frattn_layer_norm", dev, x.data_ptr(), xs, _ptr(weight), _ptr(bias), _DT[pd], T, C, eps,
-          _DT[x.dtype], out.data_ptr(), os, _ptr(mean), _ptr(rstd))
-    return (out, mean, rstd) if return_stats else out
+    if not return_stats:
+        _call("frattn_layer_norm", dev, x.data_ptr(), xs, wp, bp, _DT[pd], T, C, eps, _DT[dt], out.data_ptr(), os, None, None)
+        return out
+    mean = torch.empty(T, dtype=torch.float32, device=dev)
+    rstd = torch.empty_like(mean)
+    _call("frattn_layer_norm", dev, x.data_ptr(), xs, wp, bp, _DT[pd], T, C, eps, _DT[dt], out.data_ptr(), os,
+          mean.data_ptr(), rstd.data_ptr())
+    return out, mean, rstd
 
 
 def layer_norm_backward(
