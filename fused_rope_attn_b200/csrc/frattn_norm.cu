@@ -718,10 +718,18 @@ __global__ void __launch_bounds__(1024) column_finish_kernel(const FinishParams 
   griddep_wait();
   griddep_launch_dependents();
   float s = 0.f;
-  if (c < p.C)
-#pragma unroll 8
-    for (int g = threadIdx.y; g < p.groups; g += 32)
-      s += __ldcg(p.partial + (static_cast<size_t>(g) * p.arrays + a) * p.C + c);
+  if (c < p.C) {
+    for (int g0 = threadIdx.y; g0 < p.groups; g0 += 32 * 8) {
+      float v[8];  // (all in flight together)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int g = g0 + 32 * i;
+        v[i] = g < p.groups ? __ldcg(p.partial + (static_cast<size_t>(g) * p.arrays + a) * p.C + c) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
+  }
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   // one warp per column: lane g holds row lane g's sum
