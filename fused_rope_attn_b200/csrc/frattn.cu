@@ -376,7 +376,7 @@ int frattn_version(void) { return 100; }
 const char* frattn_error_string(int code) {
   switch (code) {
     case FRATTN_OK: return "ok";
-    case FRATTN_E_SHAPE: return "invalid shape (T, H, D or nseg)";
+    case FRATTN_E_SHAPE: return "invalid shape (T, H, D or nseg; rows, widths or strides of the block operators)";
     case FRATTN_E_DTYPE: return "unsupported element type";
     case FRATTN_E_ALIGN: return "pointer not 16-byte aligned";
     case FRATTN_E_NULL: return "required pointer is NULL";

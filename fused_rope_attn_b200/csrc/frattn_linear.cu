@@ -3,6 +3,21 @@
 //
 //   z = x W^T + b, out = act(z) + residual
 //   dz = dout act'(z); dx = dz W, dw = dz^T x, db = sum over rows of dz
+//
+// Three products on the tensor cores (tcgen05, fp32 sums in TMEM), all through TMA with
+// 128-byte swizzle; the backward's operands that run along m or n instead of along the
+// reduction are read as they lie in memory, MN-major, with no transposed copies. Large
+// products run on CTA pairs (gemm_pair_kernel), small ones on clusters that split the
+// reduction (gemm_small_kernel). dz and db come from one pass over dout and z
+// (act_bwd_kernel); dz is rounded to 16 bits once, since the tensor cores take it so.
+//
+// Measured, bf16, kernels alone: 9216 x 1280 -> 3424 in 65 us (1.24 PFLOP/s; cuBLAS's
+// bare product 61), with gelu 74, with a packed pre-activation too 81; 9216 x 3424 ->
+// 1280 with residual 71; the main loop alone takes 55 and 62. The backward of 9216 x
+// 1280 -> 3424 with gelu_tanh takes 172 us: dz and db about 44, dx 66, dw 62. Run for
+// longer than some milliseconds these are bound by the card's power (cuBLAS's 61 us
+// become 73, 71 and 172 here become 83 and 200), so that every instruction of the
+// epilogue shows, hidden or not.
 #include "frattn_block.cuh"
 
 namespace frattn {
@@ -300,8 +315,9 @@ __device__ __forceinline__ void finish_piece(const GemmParams& p, long long m, i
 // warps each take 64 columns of a TMEM lane quarter, 32 values of a row per thread and
 // step, so a block of 32 of a packed pre-activation is one thread's. (Sixteen warps: with
 // eight of them the epilogue, not the main loop, set the pace of K = 1280 with gelu:
-// two warps to a scheduler leave most of its issue slots empty.) Waits are bounded; on a timeout the kernel records a status code, waits
-// (bounded) for its own copies and MMAs, frees TMEM and returns.
+// two warps to a scheduler leave most of its issue slots empty.) Waits are bounded; on a
+// timeout the kernel records a status code, waits (bounded) for its own copies and MMAs,
+// frees TMEM and returns.
 template <int BN, bool AMN, bool BMN, typename T>
 __global__ void __launch_bounds__(GemmCfg<BN>::THREADS, 1) gemm_pair_kernel(const __grid_constant__ GemmParams p) {
   using C = GemmCfg<BN>;

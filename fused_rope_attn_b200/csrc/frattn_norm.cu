@@ -12,15 +12,19 @@
 // Both are bound by the bytes of the rows. A team of 1 to 8 warps works on a row at a
 // time, up to 40 columns to a lane held in registers, so that a row is read from memory
 // once (fewer columns and more warps cost more instructions per value than the memory
-// leaves time for: 8 columns to a lane took 17 us where this takes 10 at 9216 x 1280).
-// The forward takes one row per team and leaves it to the scheduler to overlap them.
-// The backward is persistent, because the weight gradients stay in the registers of
-// the lane that owns the column: its rows come through a ring in shared memory of the
-// team's own, filled by asynchronous 16-byte copies, which hold no registers and,
-// being cut at 16-byte boundaries of the address and not of the row, take rows of any
-// alignment. At the end the teams of a block add their gradients through shared
-// memory, each block writes one partial row, and column_finish adds the partial
-// rows, all in a fixed order (no atomics: the same bits every run).
+// leaves time for: with 8 columns to a lane a value took 28 instructions). Teams are
+// persistent: their rows come through a ring in shared memory of the team's own, filled
+// by asynchronous 16-byte copies, which hold no registers and, being cut at 16-byte
+// boundaries of the address and not of the row, take rows of any alignment. With few
+// rows a block of more warps takes each, straight from memory. The weight gradients stay
+// in the registers of the lane that owns the column; at the end the teams of a block add
+// theirs through shared memory, each block writes one partial row, and column_finish
+// adds the partial rows, all in a fixed order (no atomics: the same bits every run).
+//
+// Measured, bf16: forward 32768 x 1280 in 30.6 us (5.5 TB/s, 0.84 of the copy rate),
+// 9216 x 1280 in 11.0 us; backward 55.7 us (4.5 TB/s) and 25.3 us, of which starting,
+// joining the gradients and adding the partial rows take 10. The backward's inner loop
+// is bound by instruction issue and shared-memory reads rather than by memory.
 #include "frattn_block.cuh"
 
 namespace frattn {
