@@ -21,8 +21,8 @@
 // theirs through shared memory, each block writes one partial row, and column_finish
 // adds the partial rows, all in a fixed order (no atomics: the same bits every run).
 //
-// Measured, bf16: forward 32768 x 1280 in 30.6 us (5.5 TB/s, 0.84 of the copy rate),
-// 9216 x 1280 in 11.0 us; backward 55.7 us (4.5 TB/s) and 25.3 us, of which starting,
+// Measured, bf16: forward 32768 x 1280 in 29.0 us (5.8 TB/s, 0.88 of the copy rate),
+// 9216 x 1280 in 11.1 us; backward 54.8 us (4.6 TB/s) and 24.8 us, of which starting,
 // joining the gradients and adding the partial rows take 10. The backward's inner loop
 // is bound by instruction issue and shared-memory reads rather than by memory.
 #include "frattn_block.cuh"
@@ -280,12 +280,15 @@ __device__ __forceinline__ void stage_param(float* to, const void* src, int f32,
   }
 }
 
+// Rows of a team's ring: one worked on, one on its way (a third measured no faster: the
+// SM's other teams have theirs on their way too).
+constexpr int kPasses = 2;
+
 // How a block's shared memory is laid out: parameters, then per team the ring and the
 // reduction's floats.
 struct NormLayout {
   int warps;   // of a team
   int teams;   // of a block
-  int passes;  // rows of the ring: one worked on, the others on their way
   int slot;    // ring bytes of a row
   int cols;                // columns that a team covers, C or more: what the rows and parameters are padded to
   int params, team_bytes;  // bytes
@@ -402,21 +405,20 @@ __global__ void __launch_bounds__(256, NU > 3 ? 3 : 4) layer_norm_fwd_kernel(con
     if (fetched < p.T) fetch_row(base + fetched * stride, bytes, base, ring + into * l.slot, team.t, team.n);
     copies_commit();
     fetched += step;
-    into = into + 1 == l.passes ? 0 : into + 1;
+    into = into + 1 == kPasses ? 0 : into + 1;
   };
-  for (int k = 0; k < l.passes; ++k) clear_tail(ring + k * l.slot, bytes, l.slot, team);
+  for (int k = 0; k < kPasses; ++k) clear_tail(ring + k * l.slot, bytes, l.slot, team);
   team.sync();
   griddep_wait();
   griddep_launch_dependents();
-  for (int k = 0; k < l.passes - 1; ++k) fetch();
+  for (int k = 0; k < kPasses - 1; ++k) fetch();
   stage_param<T, VEC>(w, p.w, p.w_f32, 1.f, p.C, l.cols);
   stage_param<T, VEC>(b, p.b, p.w_f32, 0.f, p.C, l.cols);
   __syncthreads();
   const float inv_c = 1.f / static_cast<float>(p.C);
   int at = 0;
   for (long long row = first; row < p.T; row += step) {
-    if (l.passes == 2) copies_wait<0>();
-    else copies_wait<1>();
+    copies_wait<kPasses - 2>();
     team.sync();  // the row is in the ring, and nobody reads the one before it any more
     fetch();
     const uint8_t* src = ring + at * l.slot + lead(base + row * stride);
@@ -458,7 +460,7 @@ __global__ void __launch_bounds__(256, NU > 3 ? 3 : 4) layer_norm_fwd_kernel(con
       for (int e = 0; e < 8; ++e) x[u][e] = x[u][e] * rstd * g[e] + h[e];
       unit_put<T, VEC>(out, c0, u, full, p.C, x[u]);
     }
-    at = at + 1 == l.passes ? 0 : at + 1;
+    at = at + 1 == kPasses ? 0 : at + 1;
   }
 }
 
@@ -523,9 +525,9 @@ __global__ void __launch_bounds__(384) layer_norm_bwd_kernel(const NormParams p,
     }
     copies_commit();
     fetched += step;
-    into = into + 1 == l.passes ? 0 : into + 1;
+    into = into + 1 == kPasses ? 0 : into + 1;
   };
-  for (int k = 0; k < l.passes; ++k) {
+  for (int k = 0; k < kPasses; ++k) {
     uint8_t* slot = ring + k * l.slot;
     clear_tail(slot, bytes, off_x, team);
     clear_tail(slot + off_x, xbytes, off_s - off_x, team);
@@ -533,7 +535,7 @@ __global__ void __launch_bounds__(384) layer_norm_bwd_kernel(const NormParams p,
   }
   team.sync();
   griddep_wait();
-  for (int k = 0; k < l.passes - 1; ++k) fetch();
+  for (int k = 0; k < kPasses - 1; ++k) fetch();
   stage_param<T, VEC>(w, p.w, p.w_f32, 1.f, p.C, l.cols);
   __syncthreads();
   const float inv_c = 1.f / static_cast<float>(p.C);
@@ -550,8 +552,7 @@ __global__ void __launch_bounds__(384) layer_norm_bwd_kernel(const NormParams p,
       nmean = __ldcg(p.mean + row + step);
       nrstd = __ldcg(p.rstd + row + step);
     }
-    if (l.passes == 2) copies_wait<0>();
-    else copies_wait<1>();
+    copies_wait<kPasses - 2>();
     team.sync();  // the row is in the ring, and nobody reads the one before it any more
     fetch();
     const uint8_t* slot = ring + at * l.slot;
@@ -622,7 +623,7 @@ __global__ void __launch_bounds__(384) layer_norm_bwd_kernel(const NormParams p,
       for (int e = 0; e < 4; ++e) f2unpack(mul2(fma2(h[e], c2, add2(g[e], c1)), rstd2), o[2 * e], o[2 * e + 1]);
       unit_put<T, VEC>(out, c0, u, full, p.C, o);
     }
-    at = at + 1 == l.passes ? 0 : at + 1;
+    at = at + 1 == kPasses ? 0 : at + 1;
   }
   if (!p.partial) return;
   // the block's teams add their columns' sums: each in its own part of shared memory
@@ -888,17 +889,16 @@ int bwd_team_warps(int C, int vec, bool packed) {
   const int w = (C + 1023) / 1024;
   return w < 8 ? w : 8;
 }
-// With this few rows to an SM latency counts: 8 columns to a lane, up to 8 warps.
-constexpr int kFewRows = 2;
+// With this few rows to an SM latency counts: 8 columns to a lane, up to 8 warps (forward
+// of 500 x 6000: 7 us against 12 through the ring).
+constexpr int kFewRows = 2, kFewRowsFwd = 4;
 int short_team_warps(int C) {
   const int w = (C + 255) / 256;
   return w < 8 ? w : 8;
 }
 
-// Teams of a block and rows of their rings: as many teams as fit `threads` and the shared
-// memory of 1 / blocks_per_sm of an SM with rings of three rows, unless fewer than half
-// of them do (then two rows); of these no more than the rows, dealt out evenly, keep
-// busy to the end.
+// Teams of a block: as many as fit `threads` and the shared memory of 1 / blocks_per_sm of
+// an SM; of these no more than the rows, dealt out evenly, keep busy to the end.
 template <typename F>
 NormLayout norm_layout(int T, int C, int warps, int threads, int blocks_per_sm, int params, int least_team_bytes,
                        F&& slot_of_cols) {
@@ -909,12 +909,8 @@ NormLayout norm_layout(int T, int C, int warps, int threads, int blocks_per_sm, 
   l.slot = slot_of_cols(l.cols);
   const int most = threads / (32 * warps) < 15 || warps == 1 ? threads / (32 * warps) : 15;  // (named barriers 1 to 15)
   const int room = kSmemPerSm / blocks_per_sm - 1024 - l.params;
-  auto bytes = [&](int passes) {
-    const int b = passes * l.slot > least_team_bytes ? passes * l.slot : least_team_bytes;
-    return (b + 15) / 16 * 16 + 64;  // + the reduction's floats
-  };
-  l.passes = 2 * (room / bytes(3)) >= most ? 3 : 2;
-  l.team_bytes = bytes(l.passes);
+  const int ring = kPasses * l.slot > least_team_bytes ? kPasses * l.slot : least_team_bytes;
+  l.team_bytes = (ring + 15) / 16 * 16 + 64;  // + the reduction's floats
   const int fit = room / l.team_bytes;
   l.teams = most < fit ? most : fit;
   if (l.teams < 1) l.teams = 1;
@@ -951,7 +947,7 @@ int norm_fwd(NormParams p, cudaStream_t st) {
   RowVec rv(p.C, sizeof(T));
   rv.row(p.x, p.x_stride).row(p.out, p.out_stride);
   if (rv.v == 2) rv.v = 1;
-  if (p.T <= kFewRows * sms()) {
+  if (p.T <= kFewRowsFwd * sms()) {
     p.w_vec = aligned_to(p.w, 16) && aligned_to(p.b, 16);
     const int warps = short_team_warps(p.C);
     return with_shape(rv.v, p.C, warps, [&](auto vec, auto nu) {

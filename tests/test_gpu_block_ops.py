@@ -530,3 +530,52 @@ def test_activations_over_their_whole_range(act, dt):
     _, _, gb = fr.linear_act_backward(torch.ones(1, N, dtype=dt, device=DEV), eye, z.view(N, 1).to(DEV), bad.view(1, N).to(DEV),
                                       activation=act)
     assert torch.equal(gb[keep], db[keep]) and torch.isnan(gb[7]) and gb[100] == 1
+
+
+@pytest.mark.parametrize("T", [295, 296, 297, 591, 592, 593, 1777])
+@pytest.mark.parametrize("C,dt", [(1280, BF), (1285, HF), (2600, BF), (5004, BF)])
+def test_layer_norm_either_side_of_its_rules(T, C, dt):
+    """Rows around the counts where the kernels change, widths of one to several warps: the
+    same rows give the same outputs whatever the number of rows."""
+    x, w, b, dy = norm_inputs(1777, C, dt, FF, seed=7)
+    w, b = w.to(DEV), b.to(DEV)
+    y, mean, rstd = fr.layer_norm(x[:T].to(DEV), w, b, return_stats=True)
+    ry, rm, rr = B.layer_norm(f64(x[:T]), f64(w), f64(b), 1e-6)
+    near(y, ry, dt, norm_slack(f64(x[:T]), f64(w), rr, C) + 2.0 ** -22 * np.abs(f64(b)))
+    dx, dw, db = fr.layer_norm_backward(dy[:T].to(DEV), x[:T].to(DEV), w, mean, rstd)
+    rx, rw, rb = B.layer_norm_bwd(f64(dy[:T]), f64(x[:T]), f64(w), f64(mean), f64(rstd))
+    h = (np.abs(f64(x[:T])) + np.abs(f64(mean))[:, None]) * f64(rstd)[:, None]
+    g = np.abs(f64(dy[:T]) * f64(w))
+    eps = (C + 16) * 2.0 ** -23
+    near(dx, rx, dt, eps * f64(rstd)[:, None] * (g + g.mean(1, keepdims=True) + h * (g * h).mean(1, keepdims=True)))
+    near(dw, rw, FF, (T + 8) * 2.0 ** -23 * (np.abs(f64(dy[:T])) * h).sum(0))
+    near(db, rb, FF, (T + 8) * 2.0 ** -23 * np.abs(f64(dy[:T])).sum(0))
+
+
+@pytest.mark.parametrize("T,K,N,act,save", [
+    (512, 512, 512, "gelu", "packed"), (2304, 128, 640, "silu", "full"), (4100, 640, 1288, "gelu_tanh", "packed"),
+    (300, 5120, 640, "none", "packed"), (1100, 4096, 264, "relu", "full"), (2560, 2048, 256, "gelu", None),
+])
+def test_linear_act_on_each_path(T, K, N, act, save):
+    """Sizes that take the pair kernel in whole and split tiles and the small kernel with
+    several CTAs a tile, with a residual; checked on the GPU in 64 bits."""
+    x, w, b, r = [t.to(DEV) for t in linear_inputs(T, K, N, BF, True, True, seed=9)]
+    got = fr.linear_act(x, w, b, activation=act, residual=r, save_preact=save)
+    y, kept = got if save else (got, None)
+    xd, wd = x.double(), w.double()
+    z = xd @ wd.t() + b.double()
+    slack = f64((K + 2) * 2.0 ** -23 * (xd.abs() @ wd.abs().t() + b.double().abs()))
+    zn = f64(z)
+    ry = B.act(zn, act) + f64(r)
+    near(y, ry, BF, 1.13 * slack + 2.0 ** -20 * np.abs(zn) + 2.0 ** -23 * np.abs(ry))
+    if save:
+        check_preact(kept, zn, slack, BF)
+    acc = r.clone()
+    assert torch.equal(fr.linear_act(x, w, b, activation=act, residual=acc, out=acc), y)
+    z16 = torch.randn(T, N, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(BF)
+    dx, dw, db = fr.linear_act_backward(r, x, w, z16, activation=act)
+    dz = f64(r) * (1 if act == "none" else B.act_grad(f64(z16), act))
+    d = torch.from_numpy(dz).to(DEV)
+    assert rel(dx, f64(d @ wd)) < U[BF] and rel(dw, f64(d.t() @ xd)) < U[BF]
+    near(db, dz.sum(0), BF, ((T + 2) * 2.0 ** -23 + 2.0 ** -20) * 1.13 * np.abs(f64(r)).sum(0))
+    assert last_status(DEV) == 0
