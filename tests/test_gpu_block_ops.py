@@ -555,9 +555,12 @@ def test_layer_norm_either_side_of_its_rules(T, C, dt):
 @pytest.mark.parametrize("T,K,N,act,save", [
     (512, 512, 512, "gelu", "packed"), (2304, 128, 640, "silu", "full"), (4100, 640, 1288, "gelu_tanh", "packed"),
     (300, 5120, 640, "none", "packed"), (1100, 4096, 264, "relu", "full"), (2560, 2048, 256, "gelu", None),
+    (1024, 8192, 512, "silu", "packed"), (1000, 8200, 500, "relu", "full"), (9216, 1288, 1000, "relu", None),
+    (9000, 1280, 1280, "none", "packed"),
 ])
 def test_linear_act_on_each_path(T, K, N, act, save):
-    """Sizes that take the pair kernel in whole and split tiles and the small kernel with
+    """Sizes that take the pair kernel in whole tiles and in split ones (of the forward: long
+    reductions of few tiles; of the weight gradient: many rows) and the small kernel with
     several CTAs a tile, with a residual; checked on the GPU in 64 bits."""
     x, w, b, r = [t.to(DEV) for t in linear_inputs(T, K, N, BF, True, True, seed=9)]
     got = fr.linear_act(x, w, b, activation=act, residual=r, save_preact=save)
