@@ -273,8 +273,10 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // for both (1 / a = b / (a b)): the special-function unit, a quarter as wide as the
 // others, otherwise sets the pace (derivative of gelu_tanh over 9216 x 3424: 17 us of
 // 47). Arguments are limited so that the product stays finite, at magnitudes where the
-// results are 0 or 1 to 2^-60; the limit also turns a NaN into a number, so that it
-// comes back through the factor z alone and does not reach its neighbour.
+// distribution function or the sigmoid is 0 or 1 to 2^-58; the limit also turns a NaN
+// into a number, so that it comes back through the factor z alone and does not reach its
+// neighbour. A sigmoid below that is 0, not 2^-58, where z multiplies it
+// (sigmoid_factor): z itself is not limited, and has 2^127 in bf16.
 __device__ __forceinline__ uint64_t rcp_pair(float a, float b) {
   const float r = rcp_fast(a * b);
   return f2pack(r * b, r * a);
@@ -309,6 +311,8 @@ __device__ __forceinline__ uint64_t tanh_pair(uint64_t z, uint64_t z2) {
   return sigmoid_pair(u0, u1);
 }
 constexpr float kTanhLimit = 7.4f, kSiluLimit = 41.f;  // 2^u <= 2^60
+// The sigmoid s of a z limited to [-lim, lim] as the factor of z (a NaN z keeps s)
+__device__ __forceinline__ float sigmoid_factor(float z, float s, float lim) { return z < -lim ? 0.f : s; }
 
 template <int ACT>
 __device__ __forceinline__ void act_f2(float& a, float& b) {
@@ -322,14 +326,14 @@ __device__ __forceinline__ void act_f2(float& a, float& b) {
     const uint64_t z = f2pack(limit_f(a, kTanhLimit), limit_f(b, kTanhLimit));
     float s0, s1;
     f2unpack(tanh_pair(z, mul2(z, z)), s0, s1);
-    a *= s0;
-    b *= s1;
+    a *= sigmoid_factor(a, s0, kTanhLimit);
+    b *= sigmoid_factor(b, s1, kTanhLimit);
   } else if constexpr (ACT == FRATTN_ACT_SILU) {
     float u0, u1;
     f2unpack(mul2(f2pack(limit_f(a, kSiluLimit), limit_f(b, kSiluLimit)), both(-1.4426950408889634f)), u0, u1);
     f2unpack(sigmoid_pair(u0, u1), u0, u1);
-    a *= u0;
-    b *= u1;
+    a *= sigmoid_factor(a, u0, kSiluLimit);
+    b *= sigmoid_factor(b, u1, kSiluLimit);
   } else if constexpr (ACT == FRATTN_ACT_RELU) {
     a = a > 0.f ? a : (a != a ? a : 0.f);
     b = b > 0.f ? b : (b != b ? b : 0.f);
