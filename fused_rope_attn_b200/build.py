@@ -29,6 +29,7 @@ NORM_SRC = os.path.join(CSRC, "frattn_norm.cu")
 LINEAR_SRC = os.path.join(CSRC, "frattn_linear.cu")
 DEPS = [HOST_SRC, INST_SRC, WINDOW_SRC, QKV_SRC, BWD_SRC, FP8_SRC, NORM_SRC, LINEAR_SRC, os.path.join(CSRC, "frattn_kernel.cuh"),
         os.path.join(CSRC, "frattn_ptx.cuh"), os.path.join(CSRC, "frattn_block.cuh"),
+        os.path.join(CSRC, "frattn_row_pieces.h"),
         os.path.join(ROOT, "include", "frattn.h")]
 OUT = os.path.join(HERE, "libfrattn.so")
 OBJ_DIR = os.path.join(HERE, "_build")

@@ -26,6 +26,7 @@
 // joining the gradients and adding the partial rows take 10. The backward's inner loop
 // is bound by instruction issue and shared-memory reads rather than by memory.
 #include "frattn_block.cuh"
+#include "frattn_row_pieces.h"
 
 namespace frattn {
 
@@ -82,7 +83,7 @@ __device__ __forceinline__ float param_at(const void* p, int f32, int dtype_bf16
 
 // ---------------------------------------------------------------- row ring
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, uint32_t bytes) {
-  // reads `bytes` (<= 16) of the 16, the rest of dst is zeros
+  // reads `bytes` (<= 16) of the 16, the rest of dst is zeros; dst and src 16-byte aligned
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -105,17 +106,14 @@ __device__ __forceinline__ uint32_t lead(const uint8_t* row) {
 // A team's threads (t of n) copy the row at `row` into the slot dst; nothing before
 // `base`, the matrix's first row, is read, nor past the row's end.
 __device__ __forceinline__ void fetch_row(const uint8_t* row, int bytes, const uint8_t* base, uint8_t* dst, int t, int n) {
-  const int off = static_cast<int>(lead(row)), end = off + bytes;
+  const int off = static_cast<int>(lead(row));
   const uint8_t* src = row - off;
   if (t == 0 && src < base) {
-    for (int i = off; i < 16 && i < end; ++i) dst[i] = src[i];
+    for (int i = off; i < 16 && i < off + bytes; ++i) dst[i] = src[i];
     t += n;
   }
-  uint32_t d = smem_u32(dst) + 16 * t;
-  for (int at = 16 * t; at < end + 16; at += 16 * n, d += 16 * n) {
-    const int left = end - at;
-    copy16_async(d, left > 0 ? src + at : row, left < 16 ? (left > 0 ? left : 0) : 16);
-  }
+  const uint32_t to = smem_u32(dst);
+  row_pieces(off, bytes, t, n, [&](int at, int from, int size) { copy16_async(to + at, src + from, size); });
 }
 
 // The team: `warps` warps of the block with a named barrier of their own.
