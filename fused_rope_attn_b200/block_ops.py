@@ -23,6 +23,7 @@ import functools
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .fused_attn import _DT, _status_word
@@ -337,6 +338,7 @@ class _LayerNorm(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         x, scales, weight, mean, rstd = ctx.saved_tensors
         if ctx.packed:
@@ -348,8 +350,9 @@ class _LayerNorm(torch.autograd.Function):
 
 
 def layer_norm_train(x, weight=None, bias=None, *, eps: float = 1e-6, checkpoint: bool = False) -> torch.Tensor:
-    """``layer_norm`` with gradients for x, weight and bias. With ``checkpoint`` the
-    node keeps x in 8 bits, and the gradients are those at the values so kept."""
+    """``layer_norm`` with gradients for x, weight and bias, once differentiable (a second
+    derivative through it raises). With ``checkpoint`` the node keeps x in 8 bits, and
+    the gradients are those at the values so kept."""
     return _LayerNorm.apply(x, weight, bias, eps, checkpoint)
 
 
@@ -523,6 +526,7 @@ class _LinearAct(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         weight, *kept = ctx.saved_tensors
         if ctx.packed:
@@ -539,7 +543,8 @@ class _LinearAct(torch.autograd.Function):
 
 def linear_act_train(x, weight, bias=None, *, activation: str = "none", residual=None,
                      checkpoint: bool = False) -> torch.Tensor:
-    """``linear_act`` with gradients for x, weight, bias and residual. With
-    ``checkpoint`` the node keeps x and the pre-activation in 8 bits, and the
-    gradients are those at the values so kept."""
+    """``linear_act`` with gradients for x, weight, bias and residual, once
+    differentiable (a second derivative through it raises). With ``checkpoint`` the node
+    keeps x and the pre-activation in 8 bits, and the gradients are those at the values
+    so kept."""
     return _LinearAct.apply(x, weight, bias, residual, activation, checkpoint)
