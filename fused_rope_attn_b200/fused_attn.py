@@ -25,6 +25,7 @@ import threading
 from collections import OrderedDict
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -555,7 +556,7 @@ def _bwd(q, k, v, cos, sin, cu, out, lse, dout):
 class _FusedRopeAttention(torch.autograd.Function):
     """Autograd node of ``fused_rope_attention``: the forward saves lse, the
     backward runs the sm_100a backward kernels (frattn_bwd). No gradient flows
-    to cos/sin or cu_seqlens."""
+    to cos/sin or cu_seqlens, and a second derivative raises."""
 
     @staticmethod
     def forward(ctx, q, k, v, cos, sin, cu, max_seqlen):
@@ -564,6 +565,7 @@ class _FusedRopeAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, cos, sin, cu, out, lse = ctx.saved_tensors
         dq, dk, dv = _bwd(q, k, v, cos, sin, cu, out, lse, dout)

@@ -50,3 +50,13 @@ def test_first_derivatives_with_a_graph_are_the_same():
     a = torch.autograd.grad(y.float().sum(), ps, retain_graph=True)
     c = torch.autograd.grad(y.float().sum(), ps, create_graph=True)
     assert all(torch.equal(s, t) for s, t in zip(a, c))
+
+
+def test_attention_node_refuses_a_second_derivative():
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (leaf(g, 96, 2, 64) for _ in range(3))
+    cos, sin = torch.ones(96, 32, device=DEV), torch.zeros(96, 32, device=DEV)
+    cu = torch.tensor([0, 40, 96], dtype=torch.int32, device=DEV)
+    y = fr.fused_rope_attention_train(q, k, v, cos, sin, cu) + v
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        penalty(y, v).backward()
