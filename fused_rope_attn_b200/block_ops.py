@@ -15,7 +15,8 @@ operators here; each calls hand-written sm_100a kernels through the C ABI
   the autograd nodes keep their inputs that way with ``checkpoint=True``.
 
 Matrices are ``[T, C]`` with packed columns; rows may be strided (views of wider
-buffers are read in place).
+buffers are read in place). The forms without ``_train`` record no gradient, whatever
+their inputs require; ``out=`` is written in place and its version moves on.
 """
 from __future__ import annotations
 
@@ -26,7 +27,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .fused_attn import _DT, _status_word
+from .fused_attn import _DT, _status_word, _written
 
 __all__ = [
     "ACTIVATIONS",
@@ -201,13 +202,14 @@ def unpack_activation(p: PackedActivation, *, out: torch.Tensor | None = None) -
         raise ValueError(f"dtype must be float16, bfloat16 or float32, got {p.dtype}")
     codes, scales, C, dt = p
     T, dev = scales.shape[0], codes.device
-    if out is None:
+    given = out is not None
+    if not given:
         out, os = torch.empty((T, C), dtype=dt, device=dev), C
     else:
         out = _check_out_rows(out, (T, C), torch.empty(0, dtype=dt, device=dev))
         os = _stride(out)
     _call("frattn_act_unpack", dev, codes.data_ptr(), scales.data_ptr(), T, C, _DT[dt], out.data_ptr(), os)
-    return out
+    return _written(out) if given else out
 
 
 # --------------------------------------------------------------------------- layer norm
@@ -253,19 +255,20 @@ def layer_norm(
     xs, xc = x.stride()
     if xc != 1 and C > 1:
         x, xs = x.contiguous(), C
-    if out is None:
+    given = out is not None
+    if not given:
         out, os = torch.empty((T, C), dtype=dt, device=dev), C
     else:
         out = _check_out_rows(out, (T, C), x)
         os = _stride(out)
     if not return_stats:
         _call("frattn_layer_norm", dev, x.data_ptr(), xs, wp, bp, _DT[pd], T, C, eps, _DT[dt], out.data_ptr(), os, None, None)
-        return out
+        return _written(out) if given else out
     mean = torch.empty(T, dtype=torch.float32, device=dev)
     rstd = torch.empty_like(mean)
     _call("frattn_layer_norm", dev, x.data_ptr(), xs, wp, bp, _DT[pd], T, C, eps, _DT[dt], out.data_ptr(), os,
           mean.data_ptr(), rstd.data_ptr())
-    return out, mean, rstd
+    return (_written(out) if given else out), mean, rstd
 
 
 def layer_norm_backward(
@@ -409,7 +412,8 @@ def linear_act(
         residual = _rows(residual)
     if save_preact not in (None, "none", "full", "packed"):
         raise ValueError(f"save_preact must be None, 'full' or 'packed', got {save_preact!r}")
-    if out is None:
+    given = out is not None
+    if not given:
         out, out_stride = torch.empty((T, N), dtype=dt, device=dev), N
     else:
         out = _check_out_rows(out, (T, N), x)
@@ -427,6 +431,8 @@ def linear_act(
         _call("frattn_linear_act", dev, x.data_ptr(), xs, weight.data_ptr(), ws_, _ptr(bias), _ptr(residual),
               0 if residual is None else _stride(residual), act, T, K, N, _DT[dt], out.data_ptr(), out_stride, _ptr(z), N, p.codes.data_ptr() if p is not None else None,
               p.scales.data_ptr() if p is not None else None, _ptr(ws), nbytes, _status_word(dev).data_ptr())
+    if given:
+        _written(out)
     if save_preact in (None, "none"):
         return out
     return out, (z if p is None else p)

@@ -237,6 +237,14 @@ def _check_out(out, q):
     return out
 
 
+def _written(out: torch.Tensor) -> torch.Tensor:
+    """``out``, a tensor of the caller's that a kernel wrote: its version moves on, as after
+    any in-place operation, so that autograd refuses a backward pass that needs what it held."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return out
+
+
 def _check_head_dim(hd):
     if hd not in SUPPORTED_HEAD_DIMS:
         raise ValueError(f"head_dim {hd} is not supported by the sm_100a kernel (even values up to 128)")

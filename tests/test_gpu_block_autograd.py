@@ -60,3 +60,33 @@ def test_attention_node_refuses_a_second_derivative():
     y = fr.fused_rope_attention_train(q, k, v, cos, sin, cu) + v
     with pytest.raises(RuntimeError, match="once_differentiable"):
         penalty(y, v).backward()
+
+
+def test_writing_to_a_saved_tensor_shows():
+    """out= writes in place, as any in-place operation does: a tensor that a node saved for
+    its backward pass and that is overwritten before it is an error there."""
+    g = torch.Generator().manual_seed(4)
+    x, w, b = leaf(g, 8, 64), leaf(g, 64, 64, scale=0.1), leaf(g, 64)
+    other = torch.randn(8, 64, generator=g).to(DEV, BF)
+    p = fr.pack_activation(other)
+    d = [t.detach() for t in (w, b)]
+    writes = {
+        "linear_act": lambda t: fr.linear_act(other, *d, out=t),
+        "linear_act in place": lambda t: fr.linear_act(other, *d, residual=t, out=t),
+        "layer_norm": lambda t: fr.layer_norm(other, out=t),
+        "layer_norm in place": lambda t: fr.layer_norm(t, out=t),
+        "unpack_activation": lambda t: fr.unpack_activation(p, out=t),
+    }
+    for name, write in writes.items():
+        h = fr.layer_norm_train(x)
+        y = fr.linear_act_train(h, w, b)
+        before = h._version
+        with torch.no_grad():
+            write(h.detach())
+        assert h._version > before, name
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.float().sum().backward()
+    with torch.inference_mode():  # tensors without a version are written all the same
+        t = torch.zeros(8, 64, dtype=BF, device=DEV)
+        assert fr.layer_norm(other, out=t) is t and (t != 0).any()
+    assert fr.unpack_activation(p, out=t) is t
