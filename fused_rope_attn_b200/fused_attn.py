@@ -238,8 +238,8 @@ def _check_out(out, q):
 
 
 def _written(out: torch.Tensor) -> torch.Tensor:
-    """``out``, a tensor of the caller's that a kernel wrote: its version moves on, as after
-    any in-place operation, so that autograd refuses a backward pass that needs what it held."""
+    """``out``, which a kernel wrote: its version moves on, as after any in-place operation,
+    so that autograd refuses a backward pass that needs what the caller's tensor held."""
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)
     return out
@@ -352,7 +352,7 @@ def fused_rope_attention(
                 out.data_ptr(), ws.data_ptr(), ws_bytes, _status_word(q.device).data_ptr(), stream,
             )
     _lib.check(rc, "frattn_fwd")
-    return out
+    return _written(out)
 
 
 def fused_rope_attention_pos(
@@ -403,7 +403,7 @@ def fused_rope_attention_pos(
             out.data_ptr(), ws.data_ptr(), ws_bytes, _status_word(q.device).data_ptr(), stream,
         )
     _lib.check(rc, "frattn_fwd_pos")
-    return out
+    return _written(out)
 
 
 # --------------------------------------------------------------------------- rotation in the projection
@@ -476,7 +476,7 @@ def qkv_rope_projection(
             _status_word(x.device).data_ptr(), stream,
         )
     _lib.check(rc, "frattn_qkv_rope")
-    return out
+    return _written(out)
 
 
 def fused_attention_rotated(
@@ -513,7 +513,7 @@ def fused_attention_rotated(
             _status_word(q.device).data_ptr(), stream,
         )
     _lib.check(rc, "frattn_fwd_rotated")
-    return out
+    return _written(out)
 
 
 # --------------------------------------------------------------------------- backward
@@ -660,4 +660,4 @@ def fused_rope_attention_fp8(
             _status_word(q.device).data_ptr(), torch.cuda.current_stream(q.device).cuda_stream,
         )
     _lib.check(rc, "frattn_fwd_fp8")
-    return out
+    return _written(out)

@@ -90,3 +90,24 @@ def test_writing_to_a_saved_tensor_shows():
         t = torch.zeros(8, 64, dtype=BF, device=DEV)
         assert fr.layer_norm(other, out=t) is t and (t != 0).any()
     assert fr.unpack_activation(p, out=t) is t
+
+
+def test_writing_to_a_saved_tensor_shows_for_the_attention():
+    g = torch.Generator().manual_seed(5)
+    T, H, D = 96, 2, 64
+    q, k, v = (torch.randn(T, H, D, generator=g).to(DEV, BF) for _ in range(3))
+    x, w = torch.randn(T, 64, generator=g).to(DEV, BF), torch.randn(3 * H * D, 64, generator=g).to(DEV, BF)
+    cos, sin = torch.ones(T, D // 2, device=DEV), torch.zeros(T, D // 2, device=DEV)
+    cu = torch.tensor([0, 40, T], dtype=torch.int32, device=DEV)
+    pos = torch.zeros(T, 2, dtype=torch.int32, device=DEV)
+    writes = {
+        "fused_rope_attention": lambda t: fr.fused_rope_attention(q, k, v, cos, sin, cu, out=t),
+        "fused_rope_attention_pos": lambda t: fr.fused_rope_attention_pos(q, k, v, pos, cu, max_position=1, out=t),
+        "fused_attention_rotated": lambda t: fr.fused_attention_rotated(q, k, v, cu, out=t),
+        "fused_rope_attention_fp8": lambda t: fr.fused_rope_attention_fp8(q, k, v, cos, sin, cu, out=t),
+    }
+    for name, write in writes.items():
+        t = torch.zeros(T, H, D, dtype=BF, device=DEV)
+        assert write(t) is t and t._version == 1, name
+    t = torch.zeros(T, 3, H, D, dtype=BF, device=DEV)
+    assert fr.qkv_rope_projection(x, w, None, cos, sin, H, out=t) is t and t._version == 1
