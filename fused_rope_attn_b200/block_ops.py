@@ -132,6 +132,39 @@ def _check_out_rows(out, shape, like, name="out"):
     return out
 
 
+def _bytes_of(t: torch.Tensor) -> tuple[int, int]:
+    """Addresses of t's first byte and past its last."""
+    p = t.data_ptr()
+    return p, p + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _apart(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether rows ``out`` and a matrix or vector t, neither empty, have no byte in common: one
+    ends before the other begins, or they are columns of one buffer that do not meet. (Rows
+    of different strides that interleave count as sharing.)"""
+    a, a_end = _bytes_of(out)
+    b, b_end = _bytes_of(t)
+    if a_end <= b or b_end <= a:
+        return True
+    if t.ndim != 2 or out.stride(0) * out.element_size() != t.stride(0) * t.element_size():
+        return False
+    row = out.stride(0) * out.element_size()
+    at = (b - a) % row if row > 0 else 0  # where t's columns begin in a row of out
+    return out.shape[1] * out.element_size() <= at and at + t.shape[1] * t.element_size() <= row
+
+
+def _check_apart(out, itself=None, **inputs):
+    """Refuses an ``out`` that shares memory with an input of its call (None: not given). The input
+    named ``itself`` may be exactly out: each row (or tile) of it is read before it is written."""
+    for name, t in inputs.items():
+        if t is None or _apart(out, t):
+            continue
+        if name != itself:
+            raise ValueError(f"out must not share memory with {name}")
+        if t.data_ptr() != out.data_ptr() or t.stride(0) != out.stride(0) and t.shape[0] > 1:
+            raise ValueError(f"out must be {name} itself or not share memory with it")
+
+
 # --------------------------------------------------------------------------- 8-bit checkpoints
 class PackedActivation(NamedTuple):
     """An ``[T, width]`` tensor kept in 8 bits: ``codes`` int8 ``[T, 32 * nb]`` and
@@ -208,6 +241,8 @@ def unpack_activation(p: PackedActivation, *, out: torch.Tensor | None = None) -
     else:
         out = _check_out_rows(out, (T, C), torch.empty(0, dtype=dt, device=dev))
         os = _stride(out)
+        if T:
+            _check_apart(out, codes=codes, scales=scales)
     _call("frattn_act_unpack", dev, codes.data_ptr(), scales.data_ptr(), T, C, _DT[dt], out.data_ptr(), os)
     return _written(out) if given else out
 
@@ -236,7 +271,8 @@ def layer_norm(
 
     ``weight`` and ``bias`` ``[C]`` in x's type or float32 (both the same). With
     ``return_stats`` also the fp32 ``mean`` and ``rstd`` ``[T]`` of the rows, which
-    ``layer_norm_backward`` takes.
+    ``layer_norm_backward`` takes. ``out`` may be ``x`` itself, and shares no memory with
+    the other inputs.
     """
     _check_rows("x", x, tuple(_DT))
     T, C = x.shape
@@ -261,6 +297,8 @@ def layer_norm(
     else:
         out = _check_out_rows(out, (T, C), x)
         os = _stride(out)
+        if T:
+            _check_apart(out, "x", x=x, weight=weight, bias=bias)
     if not return_stats:
         _call("frattn_layer_norm", dev, x.data_ptr(), xs, wp, bp, _DT[pd], T, C, eps, _DT[dt], out.data_ptr(), os, None, None)
         return _written(out) if given else out
@@ -393,7 +431,8 @@ def linear_act(
     ``ACTIVATIONS``. ``save_preact="full"`` also returns the pre-activation
     ``x @ weight.T + bias`` as a ``[T, N]`` tensor, ``"packed"`` as a
     ``PackedActivation``: ``(out, preact)``. ``out`` and ``residual`` may be strided
-    rows; ``out`` may be ``residual`` itself (added in place).
+    rows; ``out`` may be ``residual`` itself (added in place), and shares no memory with
+    the other inputs.
     """
     _check_rows("x", x, _LINEAR_DT)
     T, K = x.shape
@@ -426,6 +465,8 @@ def linear_act(
     if T > 0:
         x, xs = _rows16(x)
         weight, ws_ = _rows16(weight)
+        if given:
+            _check_apart(out, "residual", x=x, weight=weight, bias=bias, residual=residual)
         nbytes = _workspace_bytes(_lib.workspace_bytes_linear_act, dev, T, K, N)
         ws = _workspace(nbytes, dev) if nbytes else None
         _call("frattn_linear_act", dev, x.data_ptr(), xs, weight.data_ptr(), ws_, _ptr(bias), _ptr(residual),
