@@ -9,6 +9,8 @@ of 24 bits, 60 x 6 x 2^-24 ln 2 < 2^-15 of itself, and by ex2, rcp and the sum, 
 each: 2^-14 of the result is asked for. Where the sigmoid is below 2^-58 the result counts as zero: below
 41 x 2^-59 or 7.4 x 2^-58 in magnitude, so 2^-52 absolute is allowed besides.
 """
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -70,3 +72,36 @@ def test_an_infinite_argument_shows(act):
     z = torch.tensor([-float("inf"), float("inf"), float("nan"), 1.0, -1.0, 0.0], dtype=BF)
     y = forward(z, act)[0].cpu()
     assert torch.isnan(y[0]) and y[1] == float("inf") and torch.isnan(y[2]) and torch.isfinite(y[3:]).all()
+
+
+@pytest.mark.parametrize("T", [1, 9000])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_gelu_of_negative_values(dt, T):
+    """In the negative tail gelu is z times the small distribution function itself: within
+    2^-14 of itself before the rounding. That is the polynomial's 2^-14.8 and what rounds the
+    exponent, |z^2 / (2 ln 2)| <= 122 in 32 bits: 122 x 2.5 x 2^-24 ln 2 = 2^-16.2."""
+    z = -torch.cat([torch.logspace(-3, 0, 100), torch.linspace(1, 13, 1200)]).double().to(dt)
+    y = forward(z, "gelu", T)
+    zz = z.double().numpy()
+    cdf = np.array([0.5 * math.erfc(-v / math.sqrt(2)) for v in zz])
+    for row in (0, T - 1):
+        got = y[row].double().cpu().numpy()
+        over = np.abs(got - zz * cdf) - ((1.01 * U[dt] + 2.0 ** -14) * np.abs(zz * cdf) + TINY[dt])
+        assert (over <= 0).all(), f"gelu({zz[over.argmax()]:.4g}): worst excess {over.max():.3e}"
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_gelu_gradient_of_negative_values(dt):
+    """cdf + z pdf: each term within 2^-14 of itself, as above."""
+    z = -torch.cat([torch.logspace(-3, 0, 100), torch.linspace(1, 13, 1200)]).double().to(dt)
+    N = z.numel()
+    one = torch.ones(1, 1, dtype=dt, device=DEV)
+    _, _, db = fr.linear_act_backward(torch.ones(1, N, dtype=dt, device=DEV), one, z.view(N, 1).to(DEV),
+                                      z.view(1, N).to(DEV), activation="gelu")
+    zz = z.double().numpy()
+    cdf = np.array([0.5 * math.erfc(-v / math.sqrt(2)) for v in zz])
+    zpdf = zz * np.exp(-zz * zz / 2) / math.sqrt(2 * math.pi)
+    over = np.abs(db.double().cpu().numpy() - (cdf + zpdf)) - (
+        1.01 * U[dt] * np.abs(cdf + zpdf) + 2.0 ** -14 * (cdf + np.abs(zpdf)) + TINY[dt])
+    assert (over <= 0).all(), f"at {zz[over.argmax()]:.4g}: worst excess {over.max():.3e}"
+    assert last_status(DEV) == 0
