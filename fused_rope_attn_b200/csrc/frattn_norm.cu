@@ -954,9 +954,20 @@ int norm_fwd(NormParams p, cudaStream_t st) {
     });
   }
   const int warps = team_warps(p.C, rv.v);
-  const int blocks = (p.C + 256 * warps - 1) / (256 * warps) > 3 ? 3 : 4;  // of 256 threads to an SM, by registers
-  const NormLayout l = norm_layout(p.T, p.C, warps, 256, blocks, 2, 0,
-                                   [](int cols) { return row_slot(cols * static_cast<int>(sizeof(T))); });
+  // Blocks of 256 threads to an SM: what the registers allow, fewer where even one team's rows
+  // and the parameters take more than that share of the shared memory (16-bit rows from
+  // 5121 columns, fp32 from 4097). The rows are dealt out over the blocks that run at once:
+  // dealt out over three to an SM where two fit, 9216 x 5376 bf16 took 90 us, so 67.
+  int blocks = (p.C + 256 * warps - 1) / (256 * warps) > 3 ? 3 : 4;
+  auto layout = [&] {
+    return norm_layout(p.T, p.C, warps, 256, blocks, 2, 0,
+                       [](int cols) { return row_slot(cols * static_cast<int>(sizeof(T))); });
+  };
+  NormLayout l = layout();
+  while (blocks > 1 && l.params + l.teams * l.team_bytes > kSmemPerSm / blocks - 1024) {
+    --blocks;
+    l = layout();
+  }
   return with_shape(rv.v, p.C, warps, [&](auto vec, auto nu) {
     auto kern = layer_norm_fwd_kernel<T, decltype(vec)::value, decltype(nu)::value>;
     static unsigned long long ring_ok = 0;
