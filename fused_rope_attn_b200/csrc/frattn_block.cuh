@@ -134,11 +134,14 @@ struct RowVec {
 
 // Launch whose start overlaps the end of the kernel before it in the stream (programmatic
 // dependent launch): the block operators are short, and follow each other. Every kernel
-// launched this way executes griddep_wait() before its first access to global memory
-// (it waits until the kernels before have completed and their writes are visible), and
-// griddep_launch_dependents() once it has nothing left to set up. Its loads go to L2
-// (ld.global.cg) or through the asynchronous copies, never through the non-coherent path,
-// whose lines may be older than the writes waited for.
+// launched this way executes griddep_wait() before its first access to global memory: it
+// waits until the kernels before have completed and their writes are visible to it, to
+// plain loads too. None of its loads is read-only by declaration (__ldg, const __restrict__),
+// which would let the non-coherent path serve it with lines older than the writes waited
+// for. Most go past L1 (ld.global.cg, asynchronous copies), since they are read once;
+// the bias, the residual, misaligned parameters and rows of more than 8192 columns are
+// plain loads. griddep_launch_dependents() comes once a kernel has nothing left to set up;
+// one that does not call it (layer_norm_bwd_kernel) lets the next start when it ends.
 template <typename... P, typename... A>
 inline int launch_overlapped(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, A... args) {
   cudaLaunchAttribute attr[2];

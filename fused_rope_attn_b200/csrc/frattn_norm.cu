@@ -706,8 +706,9 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_wide_cols_kernel(const Nor
 }
 
 // out_a[c] = sum over g < groups of partial[g][a][c], a < arrays: 32 columns and
-// 32 row lanes per block, the lanes' sums joined in a fixed order. Launched while the
-// kernel that writes the partial rows still runs (programmatic dependent launch).
+// 32 row lanes per block, the lanes' sums joined in a fixed order. Behind act_bwd_kernel
+// and the wide kernels its blocks start while those still run (programmatic dependent
+// launch), behind layer_norm_bwd_kernel as that one ends.
 struct FinishParams {
   const float* partial;
   int groups, arrays, C;
