@@ -321,7 +321,8 @@ def layer_norm_backward(
 ):
     """``(dx, dweight, dbias)`` of ``layer_norm`` for the output gradient ``dout`` ``[T, C]``.
 
-    ``x`` is the forward's input or its checkpoint, ``mean`` / ``rstd`` the forward's.
+    ``x`` is the forward's input or its checkpoint, ``mean`` / ``rstd`` the forward's (of the
+    input itself, for a checkpoint too: they are not recomputed from the kept values).
     dweight and dbias come in ``weight``'s type (``param_dtype``, default x's, when
     weight is None); with ``need_param_grads=False`` they are not computed (None).
     """
@@ -392,8 +393,9 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm_train(x, weight=None, bias=None, *, eps: float = 1e-6, checkpoint: bool = False) -> torch.Tensor:
     """``layer_norm`` with gradients for x, weight and bias, once differentiable (a second
-    derivative through it raises). With ``checkpoint`` the node keeps x in 8 bits, and
-    the gradients are those at the values so kept."""
+    derivative through it raises). With ``checkpoint`` the node keeps x in 8 bits: the
+    backward pass takes the kept values with the mean and rstd of x itself, so that the
+    normalised row is off by the rounding of x alone."""
     return _LayerNorm.apply(x, weight, bias, eps, checkpoint)
 
 
