@@ -12,7 +12,7 @@
 // (act_bwd_kernel); dz is rounded to 16 bits once, since the tensor cores take it so.
 //
 // Measured, bf16, kernels alone: 9216 x 1280 -> 3424 in 65 us (1.24 PFLOP/s; cuBLAS's
-// bare product 61), with gelu 74, with a packed pre-activation too 81; 9216 x 3424 ->
+// bare product 61), with gelu 75, with a packed pre-activation too 82; 9216 x 3424 ->
 // 1280 with residual 71; the main loop alone takes 55 and 62. The backward of 9216 x
 // 1280 -> 3424 with gelu_tanh takes 172 us: dz and db about 44, dx 66, dw 62. Run for
 // longer than some milliseconds these are bound by the card's power (cuBLAS's 61 us

@@ -22,7 +22,7 @@
 // adds the partial rows, all in a fixed order (no atomics: the same bits every run).
 //
 // Measured, bf16: forward 32768 x 1280 in 29.0 us (5.8 TB/s, 0.88 of the copy rate),
-// 9216 x 1280 in 11.1 us; backward 54.8 us (4.6 TB/s) and 24.8 us, of which starting,
+// 9216 x 1280 in 10.9 us; backward 53.6 us (4.7 TB/s) and 24.3 us, of which starting,
 // joining the gradients and adding the partial rows take 10. The backward's inner loop
 // is bound by instruction issue and shared-memory reads rather than by memory.
 #include "frattn_block.cuh"

@@ -272,10 +272,12 @@ int frattn_fwd_noalloc(const void* q, const void* k, const void* v, const void* 
  *   x, out       : [T, C], dtype F32, F16 or BF16
  *   weight, bias : [C] of param_dtype (dtype or F32), or NULL (ones / zeros)
  *   mean, rstd   : [T] fp32 or NULL
+ *   out may be x itself (same pointer and stride) and otherwise shares no memory with
+ *   the inputs
  * frattn_layer_norm_bwd: with h = (x - mean) rstd and g = dout weight,
  *   dx = rstd (g - mean(g) - h mean(g h)), dweight = sum_rows dout h,
  *   dbias = sum_rows dout (either may be NULL); x as [T, C] or as a checkpoint
- *   (x NULL, codes and scales given). The sums over rows are added in a fixed
+ *   (x NULL, codes and scales given; mean and rstd are taken as given). The sums over rows are added in a fixed
  *   order. workspace >= frattn_workspace_bytes_layer_norm_bwd(T, C), 16-byte aligned. */
 int frattn_act_pack(const void* x, long long x_stride, int T, int C, int dtype, int8_t* codes,
                     uint8_t* scales, void* stream);
@@ -304,6 +306,8 @@ enum {
  *   x : [T, K], w : [N, K] (nn.Linear layout), both F16 or BF16 (dtype) with
  *       16-byte aligned rows (strides multiples of 8; FRATTN_E_ALIGN otherwise)
  *   bias : [N] or NULL, residual : [T, N] or NULL, out : [T, N], of dtype
+ *   out may be residual itself (same pointer and stride) and otherwise shares no
+ *   memory with the inputs
  *   z : [T, N] of dtype, or z_codes / z_scales (a checkpoint of z), or all NULL:
  *       where the pre-activation the backward pass needs is written
  * z is summed in fp32; act and residual are applied to the fp32 value.
