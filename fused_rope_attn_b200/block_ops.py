@@ -133,31 +133,34 @@ def _check_out_rows(out, shape, like, name="out"):
 
 
 def _bytes_of(t: torch.Tensor) -> tuple[int, int]:
-    """Addresses of t's first byte and past its last."""
-    p = t.data_ptr()
-    return p, p + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    """Addresses of the first byte of t, a matrix or a vector, and past its last."""
+    p, n, s = t.data_ptr(), t.shape, t.stride()
+    last = (n[0] - 1) * s[0] + ((n[1] - 1) * s[1] if len(n) == 2 else 0)
+    return p, p + t.element_size() * (last + 1)
 
 
-def _apart(out: torch.Tensor, t: torch.Tensor) -> bool:
-    """Whether rows ``out`` and a matrix or vector t, neither empty, have no byte in common: one
-    ends before the other begins, or they are columns of one buffer that do not meet. (Rows
-    of different strides that interleave count as sharing.)"""
-    a, a_end = _bytes_of(out)
+def _apart(out: torch.Tensor, t: torch.Tensor, span: tuple[int, int] | None = None) -> bool:
+    """Whether rows ``out`` (``span`` its addresses, where known) and a matrix or vector t,
+    neither empty, have no byte in common: one ends before the other begins, or they are
+    columns of one buffer that do not meet. (Rows of different strides that interleave
+    count as sharing.)"""
+    a, a_end = span or _bytes_of(out)
     b, b_end = _bytes_of(t)
     if a_end <= b or b_end <= a:
         return True
-    if t.ndim != 2 or out.stride(0) * out.element_size() != t.stride(0) * t.element_size():
-        return False
     row = out.stride(0) * out.element_size()
-    at = (b - a) % row if row > 0 else 0  # where t's columns begin in a row of out
+    if t.ndim != 2 or row <= 0 or row != t.stride(0) * t.element_size():
+        return False
+    at = (b - a) % row  # where t's columns begin in a row of out
     return out.shape[1] * out.element_size() <= at and at + t.shape[1] * t.element_size() <= row
 
 
 def _check_apart(out, itself=None, **inputs):
     """Refuses an ``out`` that shares memory with an input of its call (None: not given). The input
     named ``itself`` may be exactly out: each row (or tile) of it is read before it is written."""
+    span = _bytes_of(out)
     for name, t in inputs.items():
-        if t is None or _apart(out, t):
+        if t is None or _apart(out, t, span):
             continue
         if name != itself:
             raise ValueError(f"out must not share memory with {name}")
